@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/dmf_attn.h and include/dmf_adaln.h.
+"""ctypes binding of the C ABI in include/dmf_attn.h, dmf_adaln.h, dmf_step.h and dmf_int8.h.
 
 The library is the only compute path of this package: if it cannot be loaded the
 import fails; nothing falls back to PyTorch or to the CPU.
@@ -21,7 +21,7 @@ STATUS_NAMES = {
     11: "ERR_WORKSPACE", 12: "ERR_TIMEOUT", 13: "ERR_TOO_LARGE",
 }
 
-# every symbol include/dmf_attn.h and include/dmf_adaln.h declare
+# every symbol the headers in include/ declare
 EXPORTS = (
     "dmf_attn_abi_version", "dmf_attn_status_string", "dmf_attn_fwd_dual", "dmf_attn_fwd",
     "dmf_attn_bwd", "dmf_attn_bwd_static", "dmf_attn_bwd_workspace_bytes", "dmf_attn_check_status_word",
@@ -32,8 +32,11 @@ EXPORTS = (
     "dmf_ln_modulate_fwd", "dmf_ln_modulate_bwd", "dmf_adaln_bwd_workspace_bytes",
     "dmf_gate_residual_fwd", "dmf_gate_residual_bwd", "dmf_gelu",
     "dmf_step_tail",
+    "dmf_int8_quantize", "dmf_int8_rmsnorm", "dmf_int8_ln_modulate", "dmf_int8_linear", "dmf_int8_dequantize",
 )
 ADALN_BF16, ADALN_F32 = 0, 2
+INT8_BF16, INT8_FP16, INT8_F32 = 0, 1, 2
+INT8_ACTS = {None: 0, "gelu": 1, "silu": 2}
 
 
 class Tensor4(C.Structure):
@@ -149,6 +152,50 @@ class StepTailArgs(C.Structure):
     ]
 
 
+class Int8Matrix(C.Structure):
+    """dmf_int8_matrix (include/dmf_int8.h): int8 rows, element stride of a row, a scale per row."""
+    _fields_ = [("values", C.c_void_p), ("stride", C.c_int64), ("scale", C.c_void_p)]
+
+
+class Int8QuantizeArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("channels", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+        ("reserved", C.c_int32), ("x", Rows), ("out", Int8Matrix), ("stream", C.c_void_p),
+    ]
+
+
+class Int8RmsNormArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("channels", C.c_int32), ("dtype", C.c_int32),
+        ("stream_dtype", C.c_int32), ("weight_dtype", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("x", Rows), ("residual", Rows), ("sum", Rows), ("weight", C.c_void_p), ("out", Int8Matrix), ("stream", C.c_void_p),
+    ]
+
+
+class Int8LnModulateArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("channels", C.c_int32), ("stream_dtype", C.c_int32),
+        ("dtype", C.c_int32), ("mod_dtype", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("x", Rows), ("h", Rows), ("sum", Rows), ("gate", Mod), ("shift", Mod), ("scale", Mod),
+        ("out", Int8Matrix), ("stream", C.c_void_p),
+    ]
+
+
+class Int8LinearArgs(C.Structure):
+    _fields_ = [
+        ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("out_dtype", C.c_int32), ("bias_dtype", C.c_int32),
+        ("reserved", C.c_int32), ("x", Int8Matrix), ("w", Int8Matrix), ("bias", C.c_void_p), ("out", C.c_void_p),
+        ("out_stride", C.c_int64), ("status_word", C.c_void_p), ("stream", C.c_void_p),
+    ]
+
+
+class Int8DequantizeArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("channels", C.c_int32), ("out_dtype", C.c_int32), ("x", Int8Matrix), ("out", C.c_void_p),
+        ("out_stride", C.c_int64), ("stream", C.c_void_p),
+    ]
+
+
 class DmfAttnError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"dmf_attn: {STATUS_NAMES.get(status, status)}: {message}")
@@ -207,6 +254,12 @@ def load() -> C.CDLL:
         for name, args in (("dmf_ln_modulate_fwd", LnModulateArgs), ("dmf_ln_modulate_bwd", LnModulateBwdArgs),
                            ("dmf_gate_residual_fwd", GateResidualArgs), ("dmf_gate_residual_bwd", GateResidualBwdArgs),
                            ("dmf_gelu", GeluArgs)):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int
+            fn.argtypes = [C.POINTER(args)]
+        for name, args in (("dmf_int8_quantize", Int8QuantizeArgs), ("dmf_int8_rmsnorm", Int8RmsNormArgs),
+                           ("dmf_int8_ln_modulate", Int8LnModulateArgs), ("dmf_int8_linear", Int8LinearArgs),
+                           ("dmf_int8_dequantize", Int8DequantizeArgs)):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.POINTER(args)]

@@ -1,0 +1,352 @@
+"""The 8-bit inference ops against fp64: rows in 8 bits behind activations and norms, and the product of such rows.
+
+Tolerances, from the arithmetic (u = 2^-24, half a step of fp32):
+* a quantised element is the nearest integer to 127 y / a, where y and a carry the fp32 errors of what stands before: off by at
+  most 0.5 + 127 e for a relative error e of the row, with e = 2 u for the quantisation itself (127 / a, times y), and
+  - activations: exp and the division within a few u; exp(-t) within (2 + 1.2 |t|) u, and the result's share of a row's maximum is
+    below exp(-|t|) |t|, so 16 u covers it;
+  - norms: sums of C terms taken as at most C / 32 per thread and a tree of ten: (C / 32 + 10) u, twice (mean and variance), and
+    with data of standard deviation about the mean's size a factor of 4: e = 8 (C / 32 + 10) u.
+* a scale is within the same e of a / 127, plus one division.
+* a product's sum is exact; its conversion, two scales and the bias are four roundings of the terms' magnitudes, and the result is
+  rounded once to its type."""
+
+import pytest
+import torch
+
+from dmf_b200.int8 import Int8Rows, int8_linear, ln_modulate_int8, quantize_int8, rms_norm_int8
+from oracle import int8_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+BF16, FP16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _randn(*shape, dtype=F32, seed=0, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed + 7 * sum(shape))
+    return (torch.randn(*shape, device=DEV, generator=g) * std).to(dtype)
+
+
+def _check_rows(rows, y, e):
+    """rows against the fp64 rows y that were to be quantised, with relative fp32 error e in front of the quantisation"""
+    assert rows.values.dtype == torch.int8 and rows.scale.dtype == F32
+    assert rows.values.shape == y.shape and rows.scale.shape == y.shape[:-1]
+    real, scale = orc.real_rows(y)
+    assert int(rows.values.min()) >= -127
+    assert float((rows.values.double() - real).abs().max()) <= 0.5 + 127 * (e + 2 * U)
+    assert bool(((rows.scale.double() - scale).abs() <= scale * (e + 2 * U)).all())
+
+
+def _norm_error(C):
+    return 8 * (C / 32 + 10) * U
+
+
+WIDTHS = [1, 7, 8, 64, 100, 257, 384, 1000, 1152, 2040, 4608, 9000]
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("act", [None, "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, F32])
+def test_quantize(C, act, dtype):
+    for M in (1, 37):
+        x = _randn(M, C, dtype=dtype, std=2.0)
+        _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U if act else 0.0)
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("dtype,stream", [(BF16, BF16), (BF16, F32), (FP16, FP16), (F32, BF16), (F32, F32)])
+def test_rms_norm(C, dtype, stream):
+    w = 1 + _randn(C, std=0.2, seed=3)
+    for M in (1, 29):
+        x, res = _randn(M, C, dtype=dtype), _randn(M, C, dtype=stream, seed=1)
+        _check_rows(rms_norm_int8(x, w), orc.rms_norm(x, w, 1e-6)[0], _norm_error(C))
+        rows, z = rms_norm_int8(x, w.to(dtype), 1e-3, residual=res)
+        y, z_ref = orc.rms_norm(x, w.to(dtype), 1e-3, res)
+        _check_rows(rows, y, _norm_error(C))
+        assert z.dtype == stream and torch.equal(z, (res.float() + x.float()).to(stream))
+
+
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("stream,dtype,mod", [(BF16, BF16, BF16), (F32, BF16, F32), (FP16, FP16, FP16), (F32, F32, BF16)])
+def test_ln_modulate(C, stream, dtype, mod):
+    for B, L in ((1, 1), (3, 11)):
+        x, h = _randn(B, L, C, dtype=stream) + 0.5, _randn(B, L, C, dtype=dtype, seed=1)
+        mods = _randn(B, 1, 6 * C, dtype=mod, seed=2, std=0.4)
+        gate, shift, scale = mods.chunk(6, dim=-1)[2:5]          # slices of one projection, as in the block
+        if C > 1:
+            _check_rows(ln_modulate_int8(x, shift, scale), orc.ln_modulate(x, shift, scale, 1e-6)[0], _norm_error(C))
+        rows, z = ln_modulate_int8(x, shift[:, 0], scale[:, 0], 1e-2, gate=gate[:, 0], h=h)
+        y, z_ref = orc.ln_modulate(x, shift, scale, 1e-2, gate, h)
+        _check_rows(rows, y, _norm_error(C))
+        # one rounding to the stream's type, of a sum that fp32 forms with at most two
+        half = torch.finfo(stream).eps / 2
+        near = half * z_ref.abs() + 2 * U * (x.double().abs() + (gate.double() * h.double()).abs()) + 2.0 ** -25
+        assert z.dtype == stream and bool(((z.double() - z_ref).abs() <= near).all())
+
+
+def test_rows_of_zeros_tiny_values_and_large_ones():
+    x = _randn(7, 96, std=1.0)
+    x[0] = 0.0
+    x[1] *= 2.0 ** -130                      # below the limit: counts as zeros
+    x[2] *= 2.0 ** -110
+    x[3] *= 2.0 ** 120
+    x[4, 5:] = 0.0
+    rows = quantize_int8(x)
+    assert not rows.values[:2].any() and float(rows.scale[:2].abs().max()) == 0.0
+    _check_rows(Int8Rows(rows.values[2:], rows.scale[2:]), x[2:].double(), 0.0)
+    assert not rows.dequantize(F32)[:2].any()
+    z = torch.zeros(3, 64, device=DEV, dtype=BF16)
+    rms = rms_norm_int8(z, torch.ones(64, device=DEV))
+    assert not rms.values.any() and not rms.scale.any()
+    ln = ln_modulate_int8(torch.full((1, 3, 64), 2.0, device=DEV), z[:1], z[:1])        # no variance: zeros
+    assert not ln.values.any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("C", [40, 1152, 1153])
+def test_a_value_that_is_not_finite_spoils_its_row_and_no_other(bad, C):
+    x = _randn(6, C, dtype=BF16)
+    clean = x.clone()
+    x[2, C // 2] = bad
+    w, other = quantize_int8(_randn(24, C)), [0, 1, 3, 4, 5]
+    shift = torch.zeros(1, C, device=DEV, dtype=BF16)
+    for f in (quantize_int8, lambda t: quantize_int8(t, "gelu"), lambda t: quantize_int8(t, "silu"),
+              lambda t: rms_norm_int8(t, torch.ones(C, device=DEV)),
+              lambda t: Int8Rows(*(v[0] for v in ln_modulate_int8(t[None], shift, shift)))):
+        rows, ref = f(x), f(clean)
+        assert torch.isnan(rows.scale[2]) and not rows.values[2].any()
+        assert torch.isnan(rows.dequantize()[2]).all() and torch.isnan(int8_linear(rows, w)[2]).all()
+        assert torch.equal(rows.values[other], ref.values[other]) and torch.equal(rows.scale[other], ref.scale[other])
+
+
+def test_strides_and_alignments():
+    C = 384
+    big = _randn(3, 20, 3, C, dtype=BF16)
+    sliced = big[:, :, 1]                                          # strided rows
+    assert torch.equal(quantize_int8(sliced).values, quantize_int8(sliced.contiguous()).values)
+    odd = _randn(5 * (C + 3) + 1, dtype=BF16)[1:].view(5, C + 3)[:, 1:C + 1]     # odd base and pitch
+    assert torch.equal(quantize_int8(odd).values, quantize_int8(odd.contiguous()).values)
+    t = _randn(C, 9, dtype=BF16).t()                               # no unit stride
+    assert torch.equal(quantize_int8(t).values, quantize_int8(t.contiguous()).values)
+    row = _randn(C, dtype=BF16).expand(7, C)                       # one row seven times
+    rows = quantize_int8(row)
+    assert torch.equal(rows.values, quantize_int8(row.contiguous()).values)
+    one = quantize_int8(row[0])                                    # no leading dimension
+    assert one.values.shape == (C,) and one.scale.shape == () and torch.equal(one.values, rows.values[0])
+    perm = _randn(4, 5, 6, C, dtype=BF16).permute(2, 0, 1, 3)      # leading dimensions that do not collapse
+    assert torch.equal(quantize_int8(perm).values, quantize_int8(perm.contiguous()).values)
+
+
+def _random8(*shape, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed + 7 * sum(shape))
+    q = torch.randint(-128, 128, shape, device=DEV, generator=g, dtype=torch.int8)
+    scale = torch.rand(shape[:-1], device=DEV, generator=g) * 0.02 + 1e-3
+    return Int8Rows(q, scale)
+
+
+def _pitched(r, pitch=None):
+    K = r.values.shape[-1]
+    buf = torch.full((*r.values.shape[:-1], -(-K // 16) * 16 if pitch is None else pitch), 99, dtype=torch.int8, device=DEV)
+    buf[..., :K] = r.values
+    return Int8Rows(buf[..., :K], r.scale)
+
+
+def _check_linear(x, w, bias, out_dtype):
+    out = int8_linear(x, w, bias, out_dtype=out_dtype)
+    ref, size = orc.linear(x.values, x.scale, w.values, w.scale, bias)
+    assert out.shape == (*x.values.shape[:-1], w.values.shape[0]) and out.dtype == out_dtype and out.is_contiguous()
+    half = torch.finfo(out_dtype).eps / 2 if out_dtype != F32 else 0.0
+    near = ref.abs() * half + size * 4 * U * (1 + half) + 2.0 ** -25
+    assert bool(((out.double() - ref).abs() <= near).all()), float(((out.double() - ref).abs() / near).max())
+    return out
+
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 16, 1), (1, 1152, 6912), (2, 48, 130), (5, 33, 7), (16, 1152, 384), (17, 100, 129), (64, 384, 300),
+                 (128, 128, 128), (130, 1001, 258), (256, 4608, 1152), (257, 640, 513), (300, 31, 1000), (1000, 1152, 200),
+                 (2049, 144, 776), (4000, 1152, 1152)]
+
+
+@pytest.mark.parametrize("shape", LINEAR_SHAPES)
+@pytest.mark.parametrize("out_dtype", [BF16, FP16, F32])
+def test_linear(shape, out_dtype):
+    M, K, N = shape
+    x, w = _random8(M, K), _random8(N, K, seed=1)
+    bias = _randn(N, dtype=out_dtype)
+    plain = _check_linear(x, w, None, out_dtype)
+    _check_linear(_pitched(x), _pitched(w), bias, out_dtype)
+    # one result per element whatever the layout of its rows: the sums are exact
+    assert torch.equal(int8_linear(_pitched(x), _pitched(w), out_dtype=out_dtype), plain)
+    assert torch.equal(int8_linear(_pitched(x, K + 17), w, out_dtype=out_dtype), plain)
+
+
+def test_linear_is_the_same_for_a_row_alone_and_in_a_batch():
+    x, w = _pitched(_random8(700, 1152)), _pitched(_random8(1152, 1152, seed=1))
+    bias = _randn(1152)
+    whole = int8_linear(x, w, bias)
+    for lo, hi in ((0, 1), (3, 5), (100, 133), (200, 456), (0, 699)):
+        assert torch.equal(int8_linear(Int8Rows(x.values[lo:hi], x.scale[lo:hi]), w, bias), whole[lo:hi])
+
+
+def test_linear_largest_sums():
+    """every product -128 * -128 over the longest sum there may be"""
+    K = 131071
+    for M in (1, 200):
+        x = Int8Rows(torch.full((M, K), -128, dtype=torch.int8, device=DEV), torch.ones(M, device=DEV))
+        w = Int8Rows(torch.full((3, K), -128, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV))
+        assert torch.equal(int8_linear(x, w, out_dtype=F32), torch.full((M, 3), float(K * 16384), device=DEV))
+        assert torch.equal(int8_linear(_pitched(x), _pitched(w), out_dtype=F32), torch.full((M, 3), float(K * 16384), device=DEV))
+
+
+def test_linear_shapes_of_x_and_empty_batches():
+    w = _pitched(_random8(40, 64, seed=1))
+    x = _random8(2, 3, 5, 64)
+    out = int8_linear(x, w)
+    assert out.shape == (2, 3, 5, 40)
+    assert torch.equal(out[1, 2], int8_linear(Int8Rows(x.values[1, 2], x.scale[1, 2]), w))
+    one = Int8Rows(x.values[0, 0, 0], x.scale[0, 0, 0])
+    assert torch.equal(int8_linear(one, w), out[0, 0, 0])
+    none = quantize_int8(torch.empty(0, 64, device=DEV))
+    assert int8_linear(none, w).shape == (0, 40) and none.dequantize().shape == (0, 64)
+    assert rms_norm_int8(torch.empty(2, 0, 64, device=DEV), torch.ones(64, device=DEV)).values.shape == (2, 0, 64)
+    rows, z = ln_modulate_int8(torch.empty(2, 0, 64, device=DEV), *(torch.ones(2, 64, device=DEV),) * 2,
+                               gate=torch.ones(2, 64, device=DEV), h=torch.empty(2, 0, 64, device=DEV))
+    assert rows.scale.shape == (2, 0) and z.shape == (2, 0, 64)
+
+
+@pytest.mark.parametrize("C", [5, 64, 1152, 1155])
+@pytest.mark.parametrize("dtype", [BF16, FP16, F32])
+def test_dequantize(C, dtype):
+    for r in (_random8(33, C), _pitched(_random8(33, C)), _random8(2, 3, C), quantize_int8(_randn(3, 5, C))):
+        out = r.dequantize(dtype)
+        assert out.is_contiguous() and torch.equal(out, (r.values.float() * r.scale[..., None]).to(dtype))
+
+
+def test_rows_behind_the_last_one_stay_as_they_were():
+    """the C ABI on buffers that are larger than the call"""
+    import ctypes as C
+
+    from dmf_b200 import _lib
+    x, w = _pitched(_random8(130, 96)), _pitched(_random8(100, 96, seed=1))
+    out = torch.full((200, 128), 7.0, device=DEV, dtype=BF16)
+    a = _lib.Int8LinearArgs()
+    a.m, a.n, a.k, a.out_dtype = 130, 100, 96, _lib.INT8_BF16
+    a.x = _lib.Int8Matrix(x.values.data_ptr(), x.values.stride(0), x.scale.data_ptr())
+    a.w = _lib.Int8Matrix(w.values.data_ptr(), w.values.stride(0), w.scale.data_ptr())
+    a.out, a.out_stride, a.stream = out.data_ptr(), 128, torch.cuda.current_stream().cuda_stream
+    for m in (130, 5):
+        out.fill_(7.0)
+        a.m = m
+        assert _lib.load().dmf_int8_linear(C.byref(a)) == 0
+        ref = int8_linear(Int8Rows(x.values[:m], x.scale[:m]), w)
+        assert torch.equal(out[:m, :100], ref)
+        assert bool((out[m:] == 7.0).all()) and bool((out[:, 100:] == 7.0).all())
+    rows = torch.full((50, 112), 55, dtype=torch.int8, device=DEV)
+    scale = torch.full((50,), 3.0, device=DEV)
+    src = _randn(40, 100)
+    b = _lib.Int8QuantizeArgs()
+    b.batch, b.seqlen, b.channels, b.dtype = 1, 40, 100, _lib.INT8_F32
+    b.x = _lib.Rows(src.data_ptr(), 0, 100)
+    b.out = _lib.Int8Matrix(rows.data_ptr(), 112, scale.data_ptr())
+    b.stream = a.stream
+    assert _lib.load().dmf_int8_quantize(C.byref(b)) == 0
+    assert bool((rows[40:] == 55).all()) and bool((rows[:, 100:] == 55).all()) and bool((scale[40:] == 3.0).all())
+    assert torch.equal(rows[:40, :100], quantize_int8(src).values)
+
+
+def test_a_block_half_as_it_is_used():
+    """adaLN, first product, GELU, second product, gate: the ops one after the other against the same steps in fp64 on their own
+    8-bit operands, and against the layer in fp64 with the error that 8 bits have"""
+    from dmf_b200 import adaln
+    B, L, C = 2, 96, 384
+    x, h = _randn(B, L, C, dtype=BF16), _randn(B, L, C, dtype=BF16, seed=1)
+    g_a, shift, scale, g_m = (_randn(B, 1, C, dtype=BF16, seed=s, std=0.3) for s in (2, 3, 4, 5))
+    w1, w2 = _randn(4 * C, C, seed=6, std=C ** -0.5), _randn(C, 4 * C, seed=7, std=(4 * C) ** -0.5)
+    b1, b2 = _randn(4 * C, dtype=BF16, seed=8, std=0.1), _randn(C, dtype=BF16, seed=9, std=0.1)
+    q1, q2 = quantize_int8(w1), quantize_int8(w2)
+    rows, z = ln_modulate_int8(x, shift, scale, gate=g_a, h=h)
+    u = int8_linear(rows, q1, b1)
+    rows2 = quantize_int8(u, "gelu")
+    out = adaln.gate_residual(z, g_m, int8_linear(rows2, q2, b2))
+    y, z64 = orc.ln_modulate(x, shift, scale, 1e-6, g_a, h)
+    _check_rows(rows, y, _norm_error(C))
+    _check_rows(rows2, orc.act(u, "gelu"), 16 * U)
+    full = z64 + g_m.double() * (orc.act(y @ w1.double().t() + b1.double(), "gelu") @ w2.double().t() + b2.double())
+    # each of the four quantised operands is off by at most half a scale, about amax / 254 with amax below 6 standard
+    # deviations: uniform errors of (6 / 127) / sqrt(12) = 1.4 % of a standard deviation each, GELU's output 2 times that
+    assert float((out.double() - full).norm() / full.norm()) < 0.05
+
+
+def test_another_stream_and_a_graph():
+    x, w = _randn(300, 1152, dtype=BF16), quantize_int8(_randn(640, 1152))
+    ref = int8_linear(quantize_int8(x), w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = int8_linear(quantize_int8(x), w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, ref)
+    static = x.clone()
+    graphs = []
+    for _ in range(2):                       # two graphs of the same calls, replayed one after the other and together
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = int8_linear(quantize_int8(static), w)
+        graphs.append((g, o))
+    static.copy_(x * 0.5 + 1)
+    want = int8_linear(quantize_int8(static), w)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for (g, _), s in zip(graphs, streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for _, o in graphs)
+
+
+def test_two_threads_at_once():
+    import threading
+    w = quantize_int8(_randn(1152, 1152))
+    xs = [quantize_int8(_randn(m, 1152, seed=m)) for m in (1, 100, 600, 2000)]
+    refs = [int8_linear(x, w) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(x, ref):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(int8_linear(x, w), ref):
+                    bad.append(x.values.shape)
+    threads = [threading.Thread(target=work, args=p) for p in zip(xs, refs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_refusals_of_gradients_and_tangents():
+    x = _randn(4, 64).requires_grad_(True)
+    w, bias = quantize_int8(_randn(8, 64)), _randn(8).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradients"):
+        quantize_int8(x)
+    with pytest.raises(RuntimeError, match="gradients"):
+        rms_norm_int8(x, torch.ones(64, device=DEV))
+    with pytest.raises(RuntimeError, match="gradients"):
+        int8_linear(quantize_int8(x.detach()), w, bias)
+    with torch.no_grad():
+        assert not int8_linear(quantize_int8(x), w, bias).requires_grad
+    with torch.inference_mode():
+        int8_linear(quantize_int8(x), w, bias)
+    with pytest.raises(RuntimeError, match="tangents"):
+        torch.func.jvp(lambda t: quantize_int8(t).scale, (x.detach(),), (x.detach(),))
+    # an input of a transform that carries no tangent of its own
+    y, _ = torch.func.jvp(lambda t: t * quantize_int8(x.detach()).scale[:, None], (x.detach(),), (x.detach(),))
+    assert torch.equal(y, x.detach() * quantize_int8(x.detach()).scale[:, None])
+
+
+def test_compiled():
+    w = quantize_int8(_randn(48, 100))
+    x = _randn(6, 100, dtype=BF16)
+    f = lambda t: int8_linear(quantize_int8(t, "silu"), w) + 1
+    assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))
