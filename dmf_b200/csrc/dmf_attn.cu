@@ -20,33 +20,11 @@
 #include "attn_fwd_pair.cuh"
 #include "attn_launch.h"
 #include "rmsnorm.cuh"
+#include "tensor_map.h"
 
 namespace {
 
 using namespace dmf;
-
-// ---- driver entry point for tensor-map encoding (no link-time libcuda dependency) ----
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                   CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static std::atomic<EncodeTiledFn> cached{nullptr};
-  EncodeTiledFn fn = cached.load(std::memory_order_acquire);
-  if (fn != nullptr) return fn;
-  void* sym = nullptr;
-  cudaDriverEntryPointQueryResult qres;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) != cudaSuccess ||
-      qres != cudaDriverEntryPointSuccess || sym == nullptr) {
-    (void)cudaGetLastError();
-    return nullptr;
-  }
-  fn = reinterpret_cast<EncodeTiledFn>(sym);
-  cached.store(fn, std::memory_order_release);
-  return fn;
-}
 
 // ---- per-device attributes ----
 
@@ -153,18 +131,10 @@ int make_map(CUtensorMap* map, const dmf_attn_tensor& t, int dtype, int batch, i
   cuuint32_t elem_strides[4] = {1, 1, 1, 1};
   const CUtensorMapDataType dt =
       dtype == DMF_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  auto run = [&] {
+  const CUresult r = encode_in_context([&] {
     return encode(map, dt, 4, t.ptr, dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = run();
-  if (r != CUDA_SUCCESS) {
-    // a driver call: it needs the device's context current to this thread, and on a thread without a runtime call so far
-    // (an autograd worker whose memory all comes from a cache) nothing has bound it yet; cudaSetDevice does
-    int dev = -1;
-    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = run();
-    (void)cudaGetLastError();
-  }
+  });
   return r == CUDA_SUCCESS ? DMF_ATTN_OK : DMF_ATTN_ERR_TENSOR_MAP;
 }
 

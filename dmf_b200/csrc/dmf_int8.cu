@@ -3,10 +3,14 @@
 
 #include <cstring>
 
+#include "attn_launch.h"
 #include "dmf_attn.h"
 #include "dmf_int8.h"
+#include "int8_gemm_few.cuh"
+#include "int8_gemm_pair.cuh"
 #include "int8_linear.cuh"
 #include "int8_rows.cuh"
+#include "tensor_map.h"
 
 namespace {
 
@@ -157,20 +161,130 @@ int run_ln_modulate(const dmf_int8_ln_modulate_args* a) {
   return launch_rows<kRowLn>(p, rows, static_cast<cudaStream_t>(a->stream));
 }
 
-int run_linear(const dmf_int8_linear_args* a) {
-  if (a == nullptr) return DMF_ATTN_ERR_NULL;
-  if (!known_dtype(a->out_dtype) || (a->bias != nullptr && !known_dtype(a->bias_dtype))) return DMF_ATTN_ERR_DTYPE;
-  if (a->m < 0 || a->n < 1 || a->k < 1 || a->k > kMaxK) return DMF_ATTN_ERR_SHAPE;
-  int sms = 0, st = DMF_ATTN_OK;
-  if (a->m > 0) {
-    if ((st = check_matrix(a->x, a->k, false)) != DMF_ATTN_OK) return st;
-    if ((st = check_matrix(a->w, a->k, false)) != DMF_ATTN_OK) return st;
-    if (a->bias != nullptr && (st = check_pointer(a->bias, element_bytes(a->bias_dtype))) != DMF_ATTN_OK) return st;
-    if (a->out_stride < a->n) return DMF_ATTN_ERR_STRIDE;
-    if ((st = check_pointer(a->out, element_bytes(a->out_dtype))) != DMF_ATTN_OK) return st;
+// ---- the product on the tensor cores ----
+
+// rows that TMA can read: base and pitch in whole 16-byte units, rows that do not overlap
+bool tma_can_read(const dmf_int8_matrix& t, int rows, int k) {
+  return reinterpret_cast<uintptr_t>(t.values) % 16 == 0 && (rows == 1 || (t.stride % 16 == 0 && t.stride >= k));
+}
+
+// map of `rows` rows of k bytes, boxes of 128 bytes x box_rows; what a box has beyond the matrix reads as zeros
+int make_map8(CUtensorMap* map, const dmf_int8_matrix& t, int rows, int k, int box_rows) {
+  const EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) return DMF_ATTN_ERR_DEVICE;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {rows == 1 ? (static_cast<cuuint64_t>(k) + 15) / 16 * 16 : static_cast<cuuint64_t>(t.stride)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+  const CUresult r = encode_in_context([&] {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.values, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+  return r == CUDA_SUCCESS ? DMF_ATTN_OK : DMF_ATTN_ERR_TENSOR_MAP;
+}
+
+template <typename Kernel, typename... Args>
+int launch_cluster(Kernel kernel, unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return DMF_ATTN_ERR_LAUNCH;
   }
-  if ((st = sm_count_of_current_device(&sms)) != DMF_ATTN_OK) return st;
-  if (a->m == 0) return DMF_ATTN_OK;
+  return DMF_ATTN_OK;
+}
+
+template <int BN, typename T>
+int launch_pair_gemm(const Int8GemmParams& p, int sms, cudaStream_t stream) {
+  static bool allowed[64];
+  const auto kernel = int8_gemm_pair_kernel<BN, T>;
+  if (!allow_smem(kernel, Int8PairTraits<BN>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
+  const int tiles = p.tiles_m * p.tiles_n, clusters = tiles < sms / 2 ? tiles : sms / 2;
+  return launch_cluster(kernel, 2u * clusters, kInt8PairThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
+}
+
+template <int TB, typename T>
+int launch_few_gemm(const Int8GemmParams& p, int splits, cudaStream_t stream) {
+  static bool allowed[64];
+  const auto kernel = int8_gemm_few_kernel<TB, T>;
+  if (!allow_smem(kernel, Int8FewTraits<TB>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
+  return launch_cluster(kernel, static_cast<unsigned>(p.tiles_m * p.tiles_n * splits), kInt8FewThreads, Int8FewTraits<TB>::kSmemBytes,
+                        splits, stream, p, splits);
+}
+
+// How a product is cut up: on CTA pairs with tiles of 256 x bn, or (few) tiles of tb tokens x 128 channels, k over `splits` CTAs.
+struct GemmPlan {
+  bool few;
+  int tile;    // bn or tb
+  int splits;
+};
+
+GemmPlan plan_gemm(int m, int n, int k, int sms) {
+  if (m <= 256) {
+    GemmPlan g = {true, m <= 16 ? 16 : (m <= 32 ? 32 : 64), 1};
+    const int64_t tiles = static_cast<int64_t>((m + g.tile - 1) / g.tile) * ((n + 127) / 128);
+    const int k_steps = (k + 127) / 128;
+    while (g.splits < 8 && tiles * g.splits * 2 <= sms && g.splits * 2 <= k_steps) g.splits *= 2;
+    return g;
+  }
+  return {false, 256, 1};
+}
+
+template <typename T>
+int launch_gemm(const GemmPlan& g, const Int8GemmParams& p, int sms, cudaStream_t stream) {
+  if (g.few) {
+    switch (g.tile) {
+      case 16: return launch_few_gemm<16, T>(p, g.splits, stream);
+      case 32: return launch_few_gemm<32, T>(p, g.splits, stream);
+      case 64: return launch_few_gemm<64, T>(p, g.splits, stream);
+      default: return launch_few_gemm<128, T>(p, g.splits, stream);
+    }
+  }
+  switch (g.tile) {
+    case 128: return launch_pair_gemm<128, T>(p, sms, stream);
+    case 192: return launch_pair_gemm<192, T>(p, sms, stream);
+    default: return launch_pair_gemm<256, T>(p, sms, stream);
+  }
+}
+
+int run_plan(const GemmPlan& g, const dmf_int8_linear_args* a, int sms) {
+  Int8GemmParams p;
+  std::memset(&p, 0, sizeof(p));
+  int st = make_map8(&p.x_map, a->x, a->m, a->k, g.few ? g.tile : 128);
+  if (st != DMF_ATTN_OK) return st;
+  if ((st = make_map8(&p.w_map, a->w, a->n, a->k, g.few ? 128 : g.tile / 2)) != DMF_ATTN_OK) return st;
+  p.x_scale = a->x.scale; p.w_scale = a->w.scale;
+  p.bias = a->bias; p.bias_dtype = a->bias_dtype;
+  p.out = a->out; p.out_stride = a->out_stride; p.out_dtype = a->out_dtype;
+  p.out_vec = reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && a->out_stride * element_bytes(a->out_dtype) % 16 == 0;
+  p.status_word = a->status_word;
+  p.m = a->m; p.n = a->n; p.k = a->k;
+  const int64_t tiles_m = (static_cast<int64_t>(a->m) + (g.few ? g.tile : 256) - 1) / (g.few ? g.tile : 256);
+  const int64_t tiles_n = (static_cast<int64_t>(a->n) + (g.few ? 128 : g.tile) - 1) / (g.few ? 128 : g.tile);
+  if (tiles_m * tiles_n * g.splits > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;
+  p.tiles_m = static_cast<int>(tiles_m);
+  p.tiles_n = static_cast<int>(tiles_n);
+  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+  switch (a->out_dtype) {
+    case DMF_INT8_BF16: return launch_gemm<__nv_bfloat16>(g, p, sms, stream);
+    case DMF_INT8_FP16: return launch_gemm<__half>(g, p, sms, stream);
+    default: return launch_gemm<float>(g, p, sms, stream);
+  }
+}
+
+int run_gemm(const dmf_int8_linear_args* a, int sms) { return run_plan(plan_gemm(a->m, a->n, a->k, sms), a, sms); }
+
+// ---- the product of rows that TMA cannot read ----
+
+int run_linear_any(const dmf_int8_linear_args* a) {
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   const int64_t tiles_m = (static_cast<int64_t>(a->m) + kAnyTile - 1) / kAnyTile, tiles_n = (static_cast<int64_t>(a->n) + kAnyTile - 1) / kAnyTile;
   // at most 65535 blocks fit in grid y: more rows go in slices
@@ -188,6 +302,23 @@ int run_linear(const dmf_int8_linear_args* a) {
     int8_linear_any_kernel<<<grid, 256, 0, stream>>>(p);
   }
   return launched();
+}
+
+int run_linear(const dmf_int8_linear_args* a) {
+  if (a == nullptr) return DMF_ATTN_ERR_NULL;
+  if (!known_dtype(a->out_dtype) || (a->bias != nullptr && !known_dtype(a->bias_dtype))) return DMF_ATTN_ERR_DTYPE;
+  if (a->m < 0 || a->n < 1 || a->k < 1 || a->k > kMaxK) return DMF_ATTN_ERR_SHAPE;
+  int sms = 0, st = DMF_ATTN_OK;
+  if (a->m > 0) {
+    if ((st = check_matrix(a->x, a->k, false)) != DMF_ATTN_OK) return st;
+    if ((st = check_matrix(a->w, a->k, false)) != DMF_ATTN_OK) return st;
+    if (a->bias != nullptr && (st = check_pointer(a->bias, element_bytes(a->bias_dtype))) != DMF_ATTN_OK) return st;
+    if (a->out_stride < a->n) return DMF_ATTN_ERR_STRIDE;
+    if ((st = check_pointer(a->out, element_bytes(a->out_dtype))) != DMF_ATTN_OK) return st;
+  }
+  if ((st = sm_count_of_current_device(&sms)) != DMF_ATTN_OK) return st;
+  if (a->m == 0) return DMF_ATTN_OK;
+  return tma_can_read(a->x, a->m, a->k) && tma_can_read(a->w, a->n, a->k) ? run_gemm(a, sms) : run_linear_any(a);
 }
 
 int run_dequantize(const dmf_int8_dequantize_args* a) {

@@ -1,0 +1,162 @@
+// The 8-bit product for few rows: the weight is the wide operand of the tensor cores.
+//
+// A CTA computes 128 output channels of TB tokens as D[channel, token] = w x^T (tcgen05.mma of kind::i8, M = 128, N = TB); the
+// CTAs of a cluster share such a tile and split k among them, so that even one token's product has every SM read its part of the
+// weight.  Each CTA sends the other CTAs their columns of its sums (int32: exact, the order does not matter) through distributed
+// shared memory; after one cluster barrier CTA r adds up columns [r TB / S, (r + 1) TB / S), scales them and writes them, 32
+// consecutive channels of a token per warp instruction.
+#pragma once
+
+#include <type_traits>
+
+#include "int8_gemm_pair.cuh"
+
+namespace dmf {
+
+template <int TB>
+struct Int8FewTraits {
+  static constexpr int kWBytes = 128 * 128, kXBytes = TB * 128, kStageBytes = kWBytes + kXBytes;
+  static constexpr int kStages = TB == 16 ? 5 : (TB == 32 ? 4 : 3);     // two CTAs per SM
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kSumBytes = TB * 128 * 4;
+  static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAcc = 2 * kStages, kNumBars = kBarAcc + 1;
+  static constexpr int kSmemBytes = 1024 + kRingBytes + kSumBytes + kNumBars * 8 + 16;
+  static constexpr uint32_t kTmemCols = TB < 32 ? 32 : TB;
+};
+
+constexpr int kInt8FewThreads = 192;
+
+template <int TB, typename T>
+__global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __grid_constant__ Int8GemmParams p, int splits) {
+  using TR = Int8FewTraits<TB>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t s_ring = smem_u32(smem);
+  int* sums = reinterpret_cast<int*>(smem + TR::kRingBytes);     // [source CTA][column of mine][channel]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TR::kRingBytes + TR::kSumBytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + TR::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8u * static_cast<uint32_t>(i); };
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % splits, tile = static_cast<int>(blockIdx.x) / splits;
+  const int tn = tile % p.tiles_n, tm = tile / p.tiles_n;
+  const int k_steps = (p.k + 127) >> 7;
+  const int k0 = static_cast<int>(static_cast<int64_t>(k_steps) * rank / splits);
+  const int k1 = static_cast<int>(static_cast<int64_t>(k_steps) * (rank + 1) / splits);   // splits <= k_steps: never empty
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < TR::kNumBars; ++i) mbar_init(bar(i), 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(smem_u32(tmem_slot), TR::kTmemCols);
+    tmem_relinquish_alloc_permit();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (splits > 1) cluster_sync_all();  // the others' shared memory is theirs from here on
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tensor_map(&p.w_map);
+      prefetch_tensor_map(&p.x_map);
+      for (int kk = k0, cnt = 0; kk < k1; ++kk, ++cnt) {
+        const uint32_t s = cnt % TR::kStages, ph = (cnt / TR::kStages) & 1u;
+        if (!mbar_wait(bar(TR::kBarEmpty + s), ph ^ 1u, abort_flag, p.status_word, kRoleInt8Producer + TR::kBarEmpty + s)) break;
+        const uint32_t dst = s_ring + s * TR::kStageBytes;
+        mbar_arrive_expect_tx(bar(TR::kBarFull + s), TR::kStageBytes);
+        tma_load_2d(dst, &p.w_map, bar(TR::kBarFull + s), kk * 128, tn * 128);
+        tma_load_2d(dst + TR::kWBytes, &p.x_map, bar(TR::kBarFull + s), kk * 128, tm * TB);
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    constexpr uint32_t idesc = make_idesc_i8(128, TB);
+    bool ok = true;
+    for (int kk = k0, cnt = 0; kk < k1; ++kk, ++cnt) {
+      const uint32_t s = cnt % TR::kStages, ph = (cnt / TR::kStages) & 1u;
+      ok = mbar_wait(bar(TR::kBarFull + s), ph, abort_flag, p.status_word, kRoleInt8Mma + TR::kBarFull + s);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t ws = s_ring + s * TR::kStageBytes, xs = ws + TR::kWBytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        mma_i8(tmem, make_smem_desc(ws + i * 32, 16, 1024, kSwizzle128), make_smem_desc(xs + i * 32, 16, 1024, kSwizzle128), idesc,
+               (kk > k0 || i > 0) ? 1u : 0u, leader);
+      tc_commit(bar(TR::kBarEmpty + s), leader);
+    }
+    if (ok) tc_commit(bar(TR::kBarAcc), leader);
+  }
+
+  // warps 2..5: a lane has one channel
+  const int quarter = warp & 3;
+  const int channel = quarter * 32 + lane;
+  const int64_t n = static_cast<int64_t>(tn) * 128 + channel;
+  const int m0 = tm * TB;
+  T* out = static_cast<T*>(p.out) + n;
+  const bool mine = warp >= 2 && n < p.n;
+  float ws = 0.f, b = 0.f;
+  bool ok = false;
+  if (warp >= 2) {
+    if (mine) {
+      ws = p.w_scale[n];
+      b = p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n) : 0.f;
+    }
+    ok = __all_sync(0xffffffffu, mbar_wait(bar(TR::kBarAcc), 0, abort_flag, p.status_word, kRoleInt8Epilogue + TR::kBarAcc));
+    tc_fence_after_sync();
+  }
+  auto put = [&](int m, int sum) {
+    if (mine && m < p.m) {
+      const float y = fmaf(static_cast<float>(sum) * p.x_scale[m], ws, b);
+      if constexpr (std::is_same<T, float>::value) out[m * p.out_stride] = y;
+      else out[m * p.out_stride] = T(y);
+    }
+  };
+  constexpr int kChunk = TB < 32 ? TB : 32;
+  const int cols = TB / splits, shift = __ffs(cols) - 1;   // columns of a CTA: a power of two
+  const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (ok) {
+#pragma unroll
+    for (int c0 = 0; c0 < TB; c0 += kChunk) {
+      uint32_t v[kChunk];
+      if constexpr (kChunk == 16) tmem_ld_x16(lane_base + c0, v);
+      else tmem_ld_x32(lane_base + c0, v);
+      tmem_wait_ld();
+      if (splits == 1) {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) put(m0 + c0 + j, static_cast<int>(v[j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const int owner = (c0 + j) >> shift, col = (c0 + j) & (cols - 1);
+          if (m0 + c0 + j < p.m)
+            st_shared_cluster_u32(map_to_cta(smem_u32(sums + (rank * cols + col) * 128 + channel), owner), v[j]);
+        }
+      }
+    }
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync_all();                          // everybody's sums have arrived
+    if (ok)
+      for (int col = 0; col < cols; ++col) {
+        int s = 0;
+        for (int r = 0; r < splits; ++r) s += sums[(r * cols + col) * 128 + channel];
+        put(m0 + rank * cols + col, s);
+      }
+  }
+  __syncwarp();
+  int8_drain(abort_flag);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, TR::kTmemCols);
+}
+
+}  // namespace dmf
