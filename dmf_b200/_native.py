@@ -69,7 +69,8 @@ def _stub(name):
     return first_call
 
 
-_stubs = {name: _stub(name) for name in ("attn_func", "attn_qkvpacked", "rms_norm", "ln_modulate", "gate_residual", "gelu")}
+_stubs = {name: _stub(name) for name in ("attn_func", "attn_qkvpacked", "rms_norm", "ln_modulate", "gate_residual", "gelu",
+                                       "quantize_int8", "rms_norm_int8", "ln_modulate_int8", "int8_linear", "dequantize_int8")}
 globals().update(_stubs)
 
 

@@ -37,6 +37,7 @@
 
 #include "dmf_adaln.h"
 #include "dmf_attn.h"
+#include "dmf_int8.h"
 #include "dmf_step.h"
 
 namespace {
@@ -981,6 +982,270 @@ std::optional<Tensor> gelu(const Tensor& x_) {
   return put_back(y, ty, route);
 }
 
+// ---- inference in 8-bit integers ------------------------------------------------------------------------------------------
+//
+// Plain tensors outside of transforms only, nothing that asks for a derivative: the rest, and what these ops refuse, is the
+// general route's.
+
+int int8_dtype(at::ScalarType t) {
+  return t == at::kBFloat16 ? DMF_INT8_BF16 : t == at::kHalf ? DMF_INT8_FP16 : t == at::kFloat ? DMF_INT8_F32 : -1;
+}
+
+bool int8_route() {
+  const Route r = find_route();
+  return r.ok && !r.jvp;
+}
+
+// a floating tensor that the ops take, on x's device
+bool int8_takes(const Tensor& t, const Tensor& x) {
+  return plain_cuda(t) && int8_dtype(t.scalar_type()) >= 0 && t.device() == x.device() && !t._fw_grad(0).defined() &&
+         !(t.requires_grad() && at::GradMode::is_enabled());
+}
+bool int8_takes(const std::optional<Tensor>& t, const Tensor& x) { return !t.has_value() || int8_takes(*t, x); }
+
+bool fits_int(int64_t n) { return n <= 0x7fffffff; }
+
+// (..., C) as (B, L, C)
+struct RowsView {
+  Tensor held;
+  dmf_rows rows = {};
+  int64_t B = 1, L = 1, C = 0;
+};
+
+RowsView rows_view(const Tensor& x) {
+  RowsView v;
+  const int64_t d = x.dim();
+  v.C = x.size(d - 1);
+  v.held = x;
+  if (d == 3) {
+    v.B = x.size(0);
+    v.L = x.size(1);
+  } else {
+    v.L = x.numel() / v.C;
+  }
+  if (x.stride(d - 1) == 1 && (d == 3 || d == 2)) {
+    v.rows = {x.data_ptr(), d == 3 ? x.stride(0) : 0, x.stride(d - 2)};
+  } else {
+    v.held = x.contiguous();
+    v.rows = {v.held.data_ptr(), v.L * v.C, v.C};
+  }
+  return v;
+}
+
+int64_t int8_pitch(int64_t C) { return (C + 15) / 16 * 16; }
+
+// uninitialised rows in 8 bits for rows of x's shape
+struct Rows8 {
+  Tensor values, scale;
+  dmf_int8_matrix m = {};
+};
+
+Rows8 empty_rows8(const Tensor& x) {
+  Rows8 r;
+  const int64_t d = x.dim(), pitch = int8_pitch(x.size(d - 1));
+  c10::SmallVector<int64_t, 8> strides(d, 1);
+  int64_t step = pitch;
+  for (int64_t i = d - 2; i >= 0; --i) {
+    strides[i] = step;
+    step *= x.size(i);
+  }
+  r.values = at::empty_strided(x.sizes(), strides, x.options().dtype(at::kChar));
+  r.scale = at::empty(x.sizes().slice(0, d - 1), x.options().dtype(at::kFloat));
+  r.m = {static_cast<int8_t*>(r.values.data_ptr()), pitch, r.scale.data_ptr<float>()};
+  return r;
+}
+
+void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
+
+bool int8_launched(int status) {
+  if (status == DMF_ATTN_OK) g_launches.fetch_add(1, std::memory_order_relaxed);
+  return status == DMF_ATTN_OK;
+}
+
+bool int8_row_shape(const Tensor& x) {
+  return x.dim() >= 1 && x.size(-1) >= 1 && x.numel() > 0 && fits_int(x.size(-1)) && fits_int(x.numel() / x.size(-1));
+}
+
+using Pair8 = std::tuple<Tensor, Tensor>;
+using Triple8 = std::tuple<Tensor, Tensor, std::optional<Tensor>>;
+
+std::optional<Pair8> quantize_int8(const Tensor& x, int64_t act) {
+  if (!int8_route() || !int8_takes(x, x) || !int8_row_shape(x)) return std::nullopt;
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const c10::cuda::CUDAGuard device_guard(x.device());
+  const RowsView v = rows_view(x);
+  const Rows8 out = empty_rows8(x);
+  dmf_int8_quantize_args a = {};
+  a.batch = v.B; a.seqlen = v.L; a.channels = v.C;
+  a.dtype = int8_dtype(x.scalar_type());
+  a.act = act;
+  a.x = v.rows;
+  a.out = out.m;
+  a.stream = stream_of(x);
+  if (!int8_launched(dmf_int8_quantize(&a))) return std::nullopt;
+  return Pair8{out.values, out.scale};
+}
+
+std::optional<Triple8> rms_norm_int8(const Tensor& x, const Tensor& weight_, double eps, const std::optional<Tensor>& residual) {
+  if (!int8_route() || !int8_takes(x, x) || !int8_takes(weight_, x) || !int8_takes(residual, x) || !int8_row_shape(x) ||
+      weight_.dim() != 1 || weight_.size(0) != x.size(-1) || (residual.has_value() && residual->sizes() != x.sizes()))
+    return std::nullopt;
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const c10::cuda::CUDAGuard device_guard(x.device());
+  const RowsView v = rows_view(x);
+  const Tensor weight = weight_.contiguous();
+  const Rows8 out = empty_rows8(x);
+  RowsView res, sum;
+  std::optional<Tensor> total;
+  dmf_int8_rmsnorm_args a = {};
+  a.batch = v.B; a.seqlen = v.L; a.channels = v.C;
+  a.dtype = int8_dtype(x.scalar_type());
+  a.weight_dtype = int8_dtype(weight.scalar_type());
+  a.eps = static_cast<float>(eps);
+  a.x = v.rows;
+  a.weight = weight.data_ptr();
+  if (residual.has_value()) {
+    total = at::empty(residual->sizes(), residual->options());
+    res = rows_view(*residual);
+    sum = rows_view(*total);
+    a.stream_dtype = int8_dtype(residual->scalar_type());
+    a.residual = res.rows;
+    a.sum = sum.rows;
+  }
+  a.out = out.m;
+  a.stream = stream_of(x);
+  if (!int8_launched(dmf_int8_rmsnorm(&a))) return std::nullopt;
+  return Triple8{out.values, out.scale, total};
+}
+
+// a (B, C) or (B, 1, C) modulation tensor of x (B, L, C)
+bool int8_mod_fits(const Tensor& t, const Tensor& x) {
+  const int64_t d = t.dim();
+  return (d == 2 || (d == 3 && t.size(1) == 1)) && t.size(0) == x.size(0) && t.size(d - 1) == x.size(2);
+}
+dmf_mod int8_mod(const Tensor& t_, at::ScalarType dtype, Tensor* held) {
+  *held = t_.scalar_type() == dtype ? t_ : t_.to(dtype);
+  if (held->stride(-1) != 1) *held = held->contiguous();
+  return {held->data_ptr(), held->stride(0)};
+}
+
+std::optional<Triple8> ln_modulate_int8(const Tensor& x, const Tensor& shift, const Tensor& scale, double eps,
+                                        const std::optional<Tensor>& gate, const std::optional<Tensor>& h) {
+  if (!int8_route() || !int8_takes(x, x) || !int8_takes(shift, x) || !int8_takes(scale, x) || !int8_takes(gate, x) || !int8_takes(h, x) ||
+      x.dim() != 3 || !int8_row_shape(x) || !int8_mod_fits(shift, x) || !int8_mod_fits(scale, x) || gate.has_value() != h.has_value() ||
+      (gate.has_value() && (!int8_mod_fits(*gate, x) || h->sizes() != x.sizes())))
+    return std::nullopt;
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const c10::cuda::CUDAGuard device_guard(x.device());
+  at::ScalarType md = shift.scalar_type();  // the kernel reads the three as one type
+  if (scale.scalar_type() != md || (gate.has_value() && gate->scalar_type() != md)) md = at::kFloat;
+  Tensor held_shift, held_scale, held_gate;
+  const RowsView v = rows_view(x);
+  RowsView hv, sum;
+  const Rows8 out = empty_rows8(x);
+  std::optional<Tensor> total;
+  dmf_int8_ln_modulate_args a = {};
+  a.batch = v.B; a.seqlen = v.L; a.channels = v.C;
+  a.stream_dtype = int8_dtype(x.scalar_type());
+  a.mod_dtype = int8_dtype(md);
+  a.eps = static_cast<float>(eps);
+  a.x = v.rows;
+  a.shift = int8_mod(shift, md, &held_shift);
+  a.scale = int8_mod(scale, md, &held_scale);
+  if (h.has_value()) {
+    total = at::empty(x.sizes(), x.options());
+    hv = rows_view(*h);
+    sum = rows_view(*total);
+    a.dtype = int8_dtype(h->scalar_type());
+    a.gate = int8_mod(*gate, md, &held_gate);
+    a.h = hv.rows;
+    a.sum = sum.rows;
+  }
+  a.out = out.m;
+  a.stream = stream_of(x);
+  if (!int8_launched(dmf_int8_ln_modulate(&a))) return std::nullopt;
+  return Triple8{out.values, out.scale, total};
+}
+
+bool is_rows8(const Tensor& values, const Tensor& scale) {
+  return plain_cuda(values) && plain_cuda(scale) && values.scalar_type() == at::kChar && values.dim() >= 1 && values.size(-1) >= 1 &&
+         int8_takes(scale, values) && scale.scalar_type() == at::kFloat &&
+         scale.sizes() == values.sizes().slice(0, values.dim() - 1);
+}
+
+// (..., K) as rows of one pitch
+struct MatrixView {
+  Tensor values, scale;
+  dmf_int8_matrix m = {};
+  int64_t rows = 1, k = 0;
+};
+
+MatrixView matrix_view(const Tensor& values, const Tensor& scale) {
+  MatrixView v;
+  const int64_t d = values.dim();
+  v.k = values.size(d - 1);
+  v.rows = values.numel() / v.k;
+  v.scale = scale.contiguous();
+  bool one_pitch = values.stride(d - 1) == 1 && d >= 2;
+  for (int64_t i = 0; i + 2 < d; ++i)
+    one_pitch = one_pitch && values.stride(i) == values.stride(i + 1) * values.size(i + 1);
+  v.values = one_pitch ? values : values.contiguous();
+  v.m = {static_cast<int8_t*>(v.values.data_ptr()), one_pitch ? values.stride(d - 2) : v.k, v.scale.data_ptr<float>()};
+  return v;
+}
+
+std::optional<Tensor> int8_linear(const Tensor& xq, const Tensor& x_scale, const Tensor& wq, const Tensor& w_scale,
+                                  const std::optional<Tensor>& bias_, at::ScalarType out_dtype) {
+  if (!int8_route() || !is_rows8(xq, x_scale) || !is_rows8(wq, w_scale) || !int8_takes(bias_, xq) || int8_dtype(out_dtype) < 0 ||
+      wq.dim() != 2 || wq.device() != xq.device() || wq.size(1) != xq.size(-1) || wq.size(0) < 1 || xq.numel() == 0 ||
+      !fits_int(wq.size(0)) || !fits_int(wq.size(1)) || !fits_int(xq.numel() / xq.size(-1)) ||
+      (bias_.has_value() && (bias_->dim() != 1 || bias_->size(0) != wq.size(0))))
+    return std::nullopt;
+  int32_t* status_word = g_status_word[xq.get_device()].load(std::memory_order_acquire);
+  if (status_word == nullptr) return std::nullopt;
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const c10::cuda::CUDAGuard device_guard(xq.device());
+  const MatrixView x = matrix_view(xq, x_scale), w = matrix_view(wq, w_scale);
+  Tensor bias;
+  c10::SmallVector<int64_t, 8> shape(xq.sizes().begin(), xq.sizes().end());
+  shape.back() = w.rows;
+  const Tensor out = at::empty(shape, xq.options().dtype(out_dtype));
+  dmf_int8_linear_args a = {};
+  a.m = x.rows; a.n = w.rows; a.k = x.k;
+  a.out_dtype = int8_dtype(out_dtype);
+  a.x = x.m;
+  a.w = w.m;
+  if (bias_.has_value()) {
+    bias = bias_->contiguous();
+    a.bias = bias.data_ptr();
+    a.bias_dtype = int8_dtype(bias.scalar_type());
+  }
+  a.out = out.data_ptr();
+  a.out_stride = w.rows;
+  a.status_word = status_word;
+  a.stream = stream_of(xq);
+  if (!int8_launched(dmf_int8_linear(&a))) return std::nullopt;
+  return out;
+}
+
+std::optional<Tensor> dequantize_int8(const Tensor& q, const Tensor& scale, at::ScalarType dtype) {
+  if (!int8_route() || !is_rows8(q, scale) || int8_dtype(dtype) < 0 || q.numel() == 0 || !fits_int(q.size(-1))) return std::nullopt;
+  at::AutoDispatchBelowADInplaceOrView below_autograd;
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  const MatrixView v = matrix_view(q, scale);
+  const Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
+  dmf_int8_dequantize_args a = {};
+  a.rows = v.rows;
+  a.channels = v.k;
+  a.out_dtype = int8_dtype(dtype);
+  a.x = v.m;
+  a.out = out.data_ptr();
+  a.out_stride = v.k;
+  a.stream = stream_of(q);
+  if (!int8_launched(dmf_int8_dequantize(&a))) return std::nullopt;
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dmf_torch, m) {
@@ -991,6 +1256,11 @@ PYBIND11_MODULE(_dmf_torch, m) {
   m.def("ln_modulate", &ln_modulate, release());
   m.def("gate_residual", &gate_residual, release());
   m.def("gelu", &gelu, release());
+  m.def("quantize_int8", &quantize_int8, release());
+  m.def("rms_norm_int8", &rms_norm_int8, release());
+  m.def("ln_modulate_int8", &ln_modulate_int8, release());
+  m.def("int8_linear", &int8_linear, release());
+  m.def("dequantize_int8", &dequantize_int8, release());
   m.def("set_status_word", [](int64_t device, int64_t ptr) {
     TORCH_CHECK(device >= 0 && device < kMaxDevices, "device index out of range");
     g_status_word[device].store(reinterpret_cast<int32_t*>(ptr), std::memory_order_release);

@@ -24,10 +24,11 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from . import _lib
+from . import _lib, _native
 from . import ops as _ops
 
 _DTYPES = {torch.bfloat16: _lib.INT8_BF16, torch.float16: _lib.INT8_FP16, torch.float32: _lib.INT8_F32}
+MAX_ROWS, MAX_WIDTH = 2 ** 31 - 1, 2 ** 20
 MAX_K = 131071      # of a product: beyond it a sum of 8-bit products could leave int32
 
 
@@ -40,6 +41,10 @@ class Int8Rows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the rows stand for, as a contiguous (..., C) tensor of a floating type."""
+        if _native.takes(*self):
+            out = _native.dequantize_int8(*self, dtype)
+            if out is not None:
+                return out
         _check_rows8(self)
         if dtype not in _DTYPES:
             raise TypeError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
@@ -78,13 +83,14 @@ def _check_rows8(r: Int8Rows) -> None:
         raise TypeError(f"expected int8 values and fp32 scales, got {values.dtype} and {scale.dtype}")
     if values.dim() < 1 or scale.shape != values.shape[:-1] or scale.device != values.device:
         raise ValueError(f"a scale per row: values {tuple(values.shape)} on {values.device}, scale {tuple(scale.shape)} on {scale.device}")
-    if values.shape[-1] < 1:
-        raise ValueError("rows must have at least one element")
+    _check_width(values)
 
 
 def _check_width(x: torch.Tensor) -> None:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"expected rows of at least one element, got shape {tuple(x.shape)}")
+    if x.shape[-1] > MAX_WIDTH or x.numel() // x.shape[-1] > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows of at most {MAX_WIDTH} elements")
 
 
 def _mod2(t: torch.Tensor, B: int, Cn: int) -> torch.Tensor:
@@ -310,6 +316,10 @@ def quantize_int8(x: torch.Tensor, activation: Optional[str] = None) -> Int8Rows
     (out_features, in_features) this gives a scale per output channel."""
     if activation not in _lib.INT8_ACTS:
         raise ValueError(f"activation must be None, 'gelu' or 'silu', got {activation!r}")
+    if _native.takes(x):
+        out = _native.quantize_int8(x, _lib.INT8_ACTS[activation])
+        if out is not None:
+            return Int8Rows(*out)
     _check_floating(x)
     _check_width(x)
     _refuse_derivatives(x)
@@ -319,6 +329,10 @@ def quantize_int8(x: torch.Tensor, activation: Optional[str] = None) -> Int8Rows
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None):
     """``z * rsqrt(mean(z^2, -1) + eps) * weight`` in 8 bits, z = x or residual + x, for x (..., C) and weight (C).  With a
     residual returns (rows, z in the residual's type); the norm is of z before that rounding."""
+    if _native.takes(x, weight, residual):
+        out = _native.rms_norm_int8(x, weight, eps, residual)
+        if out is not None:
+            return Int8Rows(*out[:2]) if residual is None else (Int8Rows(*out[:2]), out[2])
     _check_floating(x, weight, residual)
     _check_width(x)
     if weight.shape != x.shape[-1:]:
@@ -339,6 +353,10 @@ def ln_modulate_int8(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, 
     type); the norm is of z before that rounding."""
     if (gate is None) != (h is None):
         raise ValueError("gate and h come together")
+    if _native.takes(x, shift, scale, gate, h):
+        out = _native.ln_modulate_int8(x, shift, scale, eps, gate, h)
+        if out is not None:
+            return Int8Rows(*out[:2]) if h is None else (Int8Rows(*out[:2]), out[2])
     _check_floating(x, shift, scale, gate, h)
     _check_width(x)
     if x.dim() != 3:
@@ -360,7 +378,12 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ weight.T + bias`` of rows in 8 bits: x (..., K), weight (N, K), bias (N); the result (..., N) in ``out_dtype``.
     The sums are exact, one rounding at the end."""
-    x, weight = Int8Rows(*x), Int8Rows(*weight)
+    (xq, x_scale), (wq, w_scale) = x, weight
+    if _native.takes(xq, x_scale, wq, w_scale, bias):
+        out = _native.int8_linear(xq, x_scale, wq, w_scale, bias, out_dtype)
+        if out is not None:
+            return out
+    x, weight = Int8Rows(xq, x_scale), Int8Rows(wq, w_scale)
     _check_rows8(x)
     _check_rows8(weight)
     if weight.values.dim() != 2 or weight.values.shape[1] != x.values.shape[-1] or weight.values.shape[0] < 1:

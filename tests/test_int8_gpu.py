@@ -350,3 +350,22 @@ def test_compiled():
     x = _randn(6, 100, dtype=BF16)
     f = lambda t: int8_linear(quantize_int8(t, "silu"), w) + 1
     assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))
+
+
+def test_the_registered_ops_give_the_native_paths_bits():
+    ops = torch.ops.dmf_b200
+    x, res, w = _randn(3, 40, 200, dtype=BF16), _randn(3, 40, 200, seed=1), 1 + _randn(200, std=0.1, seed=2)
+    shift, scale, gate = (_randn(3, 1, 200, dtype=BF16, seed=s, std=0.3) for s in (3, 4, 5))
+    pairs = [(quantize_int8(x, "gelu"), ops.quantize_int8(x, 1)),
+             (rms_norm_int8(x, w), ops.rms_norm_int8(x, w, 1e-6)),
+             (ln_modulate_int8(x, shift, scale), ops.ln_modulate_int8(x, shift, scale, 1e-6))]
+    rows, z = rms_norm_int8(x, w, residual=res)
+    pairs.append(((*rows, z), ops.add_rms_norm_int8(x, res, w, 1e-6)))
+    rows, z = ln_modulate_int8(x, shift, scale, gate=gate[:, 0], h=x)
+    pairs.append(((*rows, z), ops.gate_ln_modulate_int8(x, gate, x, shift, scale, 1e-6)))
+    wq, bias = quantize_int8(_randn(77, 200)), _randn(77)
+    pairs.append(((int8_linear(rows, wq, bias, out_dtype=F32),), (ops.int8_linear(*rows, *wq, bias, F32),)))
+    pairs.append(((rows.dequantize(FP16),), (ops.dequantize_int8(*rows, FP16),)))
+    for native, general in pairs:
+        for a, b in zip(native, general):
+            assert a.stride() == b.stride() and torch.equal(a, b)
