@@ -18,6 +18,8 @@
 #include <cuda.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "int8_rows.cuh"
 #include "sm100_ptx.cuh"
 
@@ -42,14 +44,14 @@ constexpr int kRoleInt8Producer = 600, kRoleInt8Mma = 700, kRoleInt8Epilogue = 8
 template <typename T>
 struct OutVec {
   static constexpr int kElems = 8;
-  __device__ __forceinline__ static uint4 pack(const float (&v)[8]) {
+  __device__ __forceinline__ static uint4 pack(const float* v) {
     return make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]), Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
   }
 };
 template <>
 struct OutVec<float> {
   static constexpr int kElems = 4;
-  __device__ __forceinline__ static uint4 pack(const float (&v)[4]) {
+  __device__ __forceinline__ static uint4 pack(const float* v) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   }
 };
@@ -184,12 +186,29 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(con
     // =========================== epilogue (each CTA) ==========================
     constexpr int kCols = BN / 2;                      // columns of a warp
     constexpr int kVec = OutVec<T>::kElems;            // results per 16 bytes
+    constexpr int kPer = kCols / 32;                   // columns of a lane's scales
     const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
     float* s_w = reinterpret_cast<float*>(vecs + ew * TR::kWarpVec);
     float* s_b = s_w + kCols;
     uint8_t* stage = out_stage + ew * TR::kWarpStage;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kCols;
-    T* out = static_cast<T*>(p.out);
+    // scales and bias of a tile's columns and the scale of this lane's row: in registers a tile ahead
+    float next_w[kPer], next_b[kPer], next_x = 0.f;
+    auto fetch = [&](int t) {
+      if (t >= tiles) return;
+      int tm, tn;
+      int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
+      const int n0 = tn * BN + half * kCols;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int n = n0 + i * 32 + lane;
+        next_w[i] = n < p.n ? p.w_scale[n] : 0.f;
+        next_b[i] = n < p.n && p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n) : 0.f;
+      }
+      const int64_t m = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32 + lane;
+      next_x = m < p.m ? p.x_scale[m] : 0.f;
+    };
+    fetch(cluster_id);
     uint32_t tcnt = 0;
     for (int t = cluster_id; t < tiles; t += num_clusters, ++tcnt) {
       int tm, tn;
@@ -197,52 +216,70 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(con
       const int n0 = tn * BN + half * kCols;
       const int64_t m0 = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32;
       const uint32_t a = tcnt & 1u;
-      for (int i = lane; i < kCols; i += 32) {
-        const bool in = n0 + i < p.n;
-        s_w[i] = in ? p.w_scale[n0 + i] : 0.f;
-        s_b[i] = in && p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n0 + i) : 0.f;
+      const float xs = next_x;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        s_w[i * 32 + lane] = next_w[i];
+        s_b[i * 32 + lane] = next_b[i];
       }
-      const float xs = m0 + lane < p.m ? p.x_scale[m0 + lane] : 0.f;
+      fetch(t + num_clusters);
       __syncwarp();
       const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(TR::kBarAccFull + a), (tcnt >> 1) & 1u, abort_flag, p.status_word,
                                                         kRoleInt8Epilogue + TR::kBarAccFull + a));
       if (!ok) break;
       tc_fence_after_sync();
+      const bool whole = p.out_vec && m0 + 32 <= p.m && n0 + kCols <= p.n;
       // W columns from column c0 of this warp: at most 128 bytes of each row go through shared memory at a time
       auto emit = [&](int c0, auto width) {
         constexpr int W = decltype(width)::value;
         constexpr int kPieces = W / kVec;              // 16-byte pieces of a row, 8 or 4
+        constexpr int kRows = 32 / kPieces;            // rows per warp-wide store
         auto slot = [](int row, int piece) -> int {
           return row * (kPieces * 16) + ((piece ^ (kPieces == 8 ? row & 7 : (row >> 1) & 3)) << 4);
         };
 #pragma unroll
         for (int h = 0; h < W / 32; ++h) {
+          const int c = c0 + h * 32;
           uint32_t v[32];
-          tmem_ld_x32(lane_base + a * BN + c0 + h * 32, v);
+          tmem_ld_x32(lane_base + a * BN + c, v);
+          float4 w4[8], b4[8];                         // under the load: all before the stores, which could alias them
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            w4[i] = *reinterpret_cast<const float4*>(s_w + c + 4 * i);
+            b4[i] = *reinterpret_cast<const float4*>(s_b + c + 4 * i);
+          }
           tmem_wait_ld();
-          if (c0 + h * 32 + 32 == kCols) {             // the tile's last read: the accumulator may be written again
+          if (c + 32 == kCols) {                       // the tile's last read: the accumulator may be written again
             tc_fence_before_sync();
             mbar_arrive_warp_cluster(lbar(TR::kBarAccEmpty + a));
           }
+          float f[32];
 #pragma unroll
-          for (int j = 0; j < 32; j += kVec) {
-            float f[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-              const int c = c0 + h * 32 + j + i;
-              f[i] = fmaf(static_cast<float>(static_cast<int>(v[j + i])) * xs, s_w[c], s_b[c]);
-            }
-            *reinterpret_cast<uint4*>(stage + slot(lane, (h * 32 + j) / kVec)) = OutVec<T>::pack(f);
+          for (int i = 0; i < 8; ++i) {
+            f[4 * i] = fmaf(static_cast<float>(static_cast<int>(v[4 * i])) * xs, w4[i].x, b4[i].x);
+            f[4 * i + 1] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 1])) * xs, w4[i].y, b4[i].y);
+            f[4 * i + 2] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 2])) * xs, w4[i].z, b4[i].z);
+            f[4 * i + 3] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 3])) * xs, w4[i].w, b4[i].w);
           }
+#pragma unroll
+          for (int j = 0; j < 32; j += kVec)
+            *reinterpret_cast<uint4*>(stage + slot(lane, (h * 32 + j) / kVec)) = OutVec<T>::pack(f + j);
         }
         __syncwarp();
+        const int row0 = lane / kPieces, piece = lane % kPieces;
+        T* dst = static_cast<T*>(p.out) + (m0 + row0) * p.out_stride + n0 + c0 + piece * kVec;
+        if (whole) {
+          uint4 v[kPieces];
 #pragma unroll
-        for (int it = 0; it < kPieces; ++it) {
-          const int row = it * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + slot(row, piece));
+          for (int it = 0; it < kPieces; ++it) v[it] = *reinterpret_cast<const uint4*>(stage + slot(it * kRows + row0, piece));
+#pragma unroll
+          for (int it = 0; it < kPieces; ++it) *reinterpret_cast<uint4*>(dst + it * kRows * p.out_stride) = v[it];
+        } else {
           const int n = n0 + c0 + piece * kVec;
-          if (m0 + row < p.m && n < p.n) {
-            T* dst = out + (m0 + row) * p.out_stride + n;
+#pragma unroll 1
+          for (int it = 0; it < kPieces; ++it, dst += kRows * p.out_stride) {
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + slot(it * kRows + row0, piece));
+            if (m0 + it * kRows + row0 >= p.m) continue;
             if (p.out_vec && n + kVec <= p.n) {
               *reinterpret_cast<uint4*>(dst) = v;
             } else {
