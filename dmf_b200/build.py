@@ -22,7 +22,7 @@ LIB = PKG / "libdmf_attn.so"
 
 HOST_SOURCE = CSRC / "torch_host.cpp"
 
-SOURCES = ["dmf_attn.cu", "attn_fwd_duo.cu", "dmf_adaln.cu", "dmf_step.cu", "dmf_int8.cu"]
+SOURCES = ["dmf_attn.cu", "attn_fwd_duo.cu", "dmf_adaln.cu", "dmf_step.cu", "dmf_int8.cu", "dmf_int8_rows.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

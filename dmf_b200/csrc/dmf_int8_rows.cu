@@ -1,0 +1,248 @@
+// C ABI of inference in 8-bit integers (include/dmf_int8.h), rows: quantisation, norms with 8-bit results, and the way back.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "dmf_attn.h"
+#include "dmf_int8.h"
+#include "int8_launch.h"
+#include "int8_rows.cuh"
+
+namespace {
+
+using namespace dmf;
+
+constexpr int kMaxChannels = 1 << 20;
+
+int check_rows(const dmf_rows& t, int dtype) {
+  if (t.stride_b < 0 || t.stride_l < 0) return DMF_ATTN_ERR_STRIDE;
+  return check_pointer(t.ptr, element_bytes(dtype));
+}
+
+int check_row_shape(int batch, int seqlen, int channels) {
+  if (batch < 0 || seqlen < 0 || channels < 1 || channels > kMaxChannels) return DMF_ATTN_ERR_SHAPE;
+  if (static_cast<int64_t>(batch) * seqlen > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;  // rows are a grid dimension
+  return DMF_ATTN_OK;
+}
+
+// ---- which kernel ----
+
+bool whole_vectors(const void* p, int dtype, int64_t stride_b, int batch, int64_t stride_l, int seqlen) {
+  const int64_t bytes = element_bytes(dtype);
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (batch == 1 || stride_b * bytes % 16 == 0) && (seqlen == 1 || stride_l * bytes % 16 == 0);
+}
+
+bool reads_vectors(const Int8RowParams& p, int op) {
+  bool ok = p.channels % 8 == 0 && whole_vectors(p.x, p.x_dtype, p.x_sb, p.batch, p.x_sl, p.seqlen) &&
+            reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.q_stride % 8 == 0);
+  if (p.add != nullptr)
+    ok = ok && whole_vectors(p.add, p.add_dtype, p.add_sb, p.batch, p.add_sl, p.seqlen) &&
+         whole_vectors(p.sum, p.sum_dtype, p.sum_sb, p.batch, p.sum_sl, p.seqlen);
+  if (op == kRowRms) ok = ok && whole_vectors(p.weight, p.mod_dtype, 0, 1, 0, 1);
+  if (op == kRowLn) {
+    ok = ok && whole_vectors(p.shift, p.mod_dtype, p.shift_sb, p.batch, 0, 1) && whole_vectors(p.scale, p.mod_dtype, p.scale_sb, p.batch, 0, 1);
+    if (p.add != nullptr) ok = ok && whole_vectors(p.gate, p.mod_dtype, p.gate_sb, p.batch, 0, 1);
+  }
+  return ok;
+}
+
+constexpr int kWarpRowEights = 160;    // a warp's registers hold rows of up to 5 x 32 eights
+
+// A warp per row where that fills the SMs with warps; the LayerNorm form, whose blocks stay within a sample, also needs a few
+// rows of a sample per block.
+bool warp_per_row(const Int8RowParams& p, int op, int sms) {
+  return p.channels / 8 <= kWarpRowEights && p.rows >= 8ll * sms && (op != kRowLn || (p.seqlen >= 8 && p.batch <= 65535));
+}
+
+// Rows of one block of the warp kernel: the vectors are staged once per block, so many, as long as every SM has a few blocks.
+int rows_per_block(int64_t samples, int64_t rows_of_sample, int sms) {
+  for (int rpb = 32; rpb > 8; rpb /= 2)
+    if (samples * ((rows_of_sample + rpb - 1) / rpb) >= 4ll * sms) return rpb;
+  return 8;
+}
+
+template <int kOp, typename TX, typename TA>
+void launch_vectors(const Int8RowParams& p, int sms, cudaStream_t stream) {
+  const int eights = p.channels / 8;
+  if (warp_per_row(p, kOp, sms)) {
+    const int64_t samples = kOp == kRowLn ? p.batch : 1, per_sample = kOp == kRowLn ? p.seqlen : p.rows;
+    const int rpb = kOp == kRowQuantize ? kRowThreads / 32 : rows_per_block(samples, per_sample, sms);
+    const dim3 grid(static_cast<unsigned>((per_sample + rpb - 1) / rpb), static_cast<unsigned>(samples));
+    if (eights <= 64) int8_row_warp_kernel<kOp, TX, TA, 2><<<grid, kRowThreads, 0, stream>>>(p, rpb);
+    else int8_row_warp_kernel<kOp, TX, TA, 5><<<grid, kRowThreads, 0, stream>>>(p, rpb);
+    return;
+  }
+  // one eight per thread for few rows, four for many: fewer threads per row then leave room for more rows on an SM
+  const bool one = eights <= 1024 && p.rows < 4ll * sms;
+  const int per = one ? 1 : 4, threads = ((eights + per - 1) / per + 31) / 32 * 32;
+  const unsigned grid = static_cast<unsigned>(p.rows);
+  if (one) int8_row_block_kernel<kOp, TX, TA, 1><<<grid, threads, 0, stream>>>(p);
+  else int8_row_block_kernel<kOp, TX, TA, 4><<<grid, threads, 0, stream>>>(p);
+}
+
+// false: a pair of types without a kernel of its own
+template <int kOp, typename TX>
+bool launch_types(const Int8RowParams& p, int sms, cudaStream_t stream) {
+  if constexpr (kOp != kRowQuantize) {
+    if (p.add != nullptr) {
+      constexpr bool kF32 = std::is_same<TX, float>::value;
+      if (p.add_dtype == DMF_INT8_F32) {
+        launch_vectors<kOp, TX, float>(p, sms, stream);
+        return true;
+      }
+      if (p.add_dtype == DMF_INT8_BF16) {
+        if constexpr (kF32 || std::is_same<TX, __nv_bfloat16>::value) {
+          launch_vectors<kOp, TX, __nv_bfloat16>(p, sms, stream);
+          return true;
+        }
+      } else {
+        if constexpr (kF32 || std::is_same<TX, __half>::value) {
+          launch_vectors<kOp, TX, __half>(p, sms, stream);
+          return true;
+        }
+      }
+      return false;
+    }
+  }
+  launch_vectors<kOp, TX, void>(p, sms, stream);
+  return true;
+}
+
+template <int kOp>
+int launch_rows(const Int8RowParams& p, cudaStream_t stream) {
+  int sms = 0, st = sm_count_of_current_device(&sms);
+  if (st != DMF_ATTN_OK) return st;
+  if (p.rows == 0) return DMF_ATTN_OK;
+  bool done = false;
+  if (reads_vectors(p, kOp) && p.channels / 8 <= 4 * block_row_threads(4)) {
+    switch (p.x_dtype) {
+      case DMF_INT8_BF16: done = launch_types<kOp, __nv_bfloat16>(p, sms, stream); break;
+      case DMF_INT8_FP16: done = launch_types<kOp, __half>(p, sms, stream); break;
+      default: done = launch_types<kOp, float>(p, sms, stream);
+    }
+  }
+  if (!done) int8_row_any_kernel<kOp><<<static_cast<unsigned>(p.rows), kRowThreads, 0, stream>>>(p);
+  return launched();
+}
+
+void set_out(Int8RowParams* p, const dmf_int8_matrix& out) {
+  p->q = out.values;
+  p->q_stride = out.stride;
+  p->row_scale = out.scale;
+}
+
+int run_quantize(const dmf_int8_quantize_args* a) {
+  if (a == nullptr) return DMF_ATTN_ERR_NULL;
+  if (!known_dtype(a->dtype)) return DMF_ATTN_ERR_DTYPE;
+  if (a->act < DMF_INT8_ACT_NONE || a->act > DMF_INT8_ACT_SILU) return DMF_ATTN_ERR_SHAPE;
+  int st = check_row_shape(a->batch, a->seqlen, a->channels);
+  if (st != DMF_ATTN_OK) return st;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->seqlen;
+  if (rows > 0) {
+    if ((st = check_rows(a->x, a->dtype)) != DMF_ATTN_OK) return st;
+    if ((st = check_matrix(a->out, a->channels, true)) != DMF_ATTN_OK) return st;
+  }
+  Int8RowParams p = {};
+  p.x = a->x.ptr; p.x_sb = a->x.stride_b; p.x_sl = a->x.stride_l; p.x_dtype = a->dtype;
+  p.rows = rows; p.batch = a->batch; p.seqlen = a->seqlen; p.channels = a->channels; p.act = a->act;
+  set_out(&p, a->out);
+  return launch_rows<kRowQuantize>(p, static_cast<cudaStream_t>(a->stream));
+}
+
+int run_rmsnorm(const dmf_int8_rmsnorm_args* a) {
+  if (a == nullptr) return DMF_ATTN_ERR_NULL;
+  if (!known_dtype(a->dtype) || !known_dtype(a->weight_dtype)) return DMF_ATTN_ERR_DTYPE;
+  const bool add = a->residual.ptr != nullptr;
+  if (add && !known_dtype(a->stream_dtype)) return DMF_ATTN_ERR_DTYPE;
+  int st = check_row_shape(a->batch, a->seqlen, a->channels);
+  if (st != DMF_ATTN_OK) return st;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->seqlen;
+  if (rows > 0) {
+    if (add != (a->sum.ptr != nullptr)) return DMF_ATTN_ERR_NULL;
+    if ((st = check_rows(a->x, a->dtype)) != DMF_ATTN_OK) return st;
+    if (add && ((st = check_rows(a->residual, a->stream_dtype)) != DMF_ATTN_OK || (st = check_rows(a->sum, a->stream_dtype)) != DMF_ATTN_OK))
+      return st;
+    if ((st = check_pointer(a->weight, element_bytes(a->weight_dtype))) != DMF_ATTN_OK) return st;
+    if ((st = check_matrix(a->out, a->channels, true)) != DMF_ATTN_OK) return st;
+  }
+  Int8RowParams p = {};
+  p.x = a->x.ptr; p.x_sb = a->x.stride_b; p.x_sl = a->x.stride_l; p.x_dtype = a->dtype;
+  p.add = a->residual.ptr; p.add_sb = a->residual.stride_b; p.add_sl = a->residual.stride_l; p.add_dtype = a->stream_dtype;
+  p.sum = a->sum.ptr; p.sum_sb = a->sum.stride_b; p.sum_sl = a->sum.stride_l; p.sum_dtype = a->stream_dtype;
+  p.weight = a->weight; p.mod_dtype = a->weight_dtype;
+  p.rows = rows; p.batch = a->batch; p.seqlen = a->seqlen; p.channels = a->channels; p.eps = a->eps;
+  set_out(&p, a->out);
+  return launch_rows<kRowRms>(p, static_cast<cudaStream_t>(a->stream));
+}
+
+int run_ln_modulate(const dmf_int8_ln_modulate_args* a) {
+  if (a == nullptr) return DMF_ATTN_ERR_NULL;
+  if (!known_dtype(a->stream_dtype) || !known_dtype(a->mod_dtype)) return DMF_ATTN_ERR_DTYPE;
+  const bool add = a->h.ptr != nullptr;
+  if (add && !known_dtype(a->dtype)) return DMF_ATTN_ERR_DTYPE;
+  int st = check_row_shape(a->batch, a->seqlen, a->channels);
+  if (st != DMF_ATTN_OK) return st;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->seqlen;
+  if (rows > 0) {
+    if (add != (a->sum.ptr != nullptr) || add != (a->gate.ptr != nullptr)) return DMF_ATTN_ERR_NULL;
+    if ((st = check_rows(a->x, a->stream_dtype)) != DMF_ATTN_OK) return st;
+    if (add && ((st = check_rows(a->h, a->dtype)) != DMF_ATTN_OK || (st = check_rows(a->sum, a->stream_dtype)) != DMF_ATTN_OK)) return st;
+    const dmf_mod* mods[] = {&a->shift, &a->scale, &a->gate};
+    for (int i = 0; i < (add ? 3 : 2); ++i) {
+      if (mods[i]->stride_b < 0) return DMF_ATTN_ERR_STRIDE;
+      if ((st = check_pointer(mods[i]->ptr, element_bytes(a->mod_dtype))) != DMF_ATTN_OK) return st;
+    }
+    if ((st = check_matrix(a->out, a->channels, true)) != DMF_ATTN_OK) return st;
+  }
+  Int8RowParams p = {};
+  p.x = a->x.ptr; p.x_sb = a->x.stride_b; p.x_sl = a->x.stride_l; p.x_dtype = a->stream_dtype;
+  p.add = a->h.ptr; p.add_sb = a->h.stride_b; p.add_sl = a->h.stride_l; p.add_dtype = a->dtype;
+  p.sum = a->sum.ptr; p.sum_sb = a->sum.stride_b; p.sum_sl = a->sum.stride_l; p.sum_dtype = a->stream_dtype;
+  p.gate = a->gate.ptr; p.gate_sb = a->gate.stride_b;
+  p.shift = a->shift.ptr; p.shift_sb = a->shift.stride_b;
+  p.scale = a->scale.ptr; p.scale_sb = a->scale.stride_b;
+  p.mod_dtype = a->mod_dtype;
+  p.rows = rows; p.batch = a->batch; p.seqlen = a->seqlen; p.channels = a->channels; p.eps = a->eps;
+  set_out(&p, a->out);
+  return launch_rows<kRowLn>(p, static_cast<cudaStream_t>(a->stream));
+}
+
+int run_dequantize(const dmf_int8_dequantize_args* a) {
+  if (a == nullptr) return DMF_ATTN_ERR_NULL;
+  if (!known_dtype(a->out_dtype)) return DMF_ATTN_ERR_DTYPE;
+  if (a->rows < 0 || a->rows > 0x7fffffff || a->channels < 1) return DMF_ATTN_ERR_SHAPE;
+  int sms = 0, st = DMF_ATTN_OK;
+  if (a->rows > 0) {
+    if ((st = check_matrix(a->x, a->channels, false)) != DMF_ATTN_OK) return st;
+    if (a->out_stride < a->channels) return DMF_ATTN_ERR_STRIDE;
+    if ((st = check_pointer(a->out, element_bytes(a->out_dtype))) != DMF_ATTN_OK) return st;
+  }
+  if ((st = sm_count_of_current_device(&sms)) != DMF_ATTN_OK) return st;
+  if (a->rows == 0) return DMF_ATTN_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+  const bool vectors = a->channels % 8 == 0 && reinterpret_cast<uintptr_t>(a->x.values) % 8 == 0 && (a->rows == 1 || a->x.stride % 8 == 0) &&
+                       whole_vectors(a->out, a->out_dtype, 0, 1, a->out_stride, a->rows == 1 ? 1 : 2);
+  if (!vectors) {
+    int8_dequantize_any_kernel<<<static_cast<unsigned>(a->rows), kRowThreads, 0, stream>>>(
+        a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->out_dtype, a->channels);
+    return launched();
+  }
+  const unsigned grid = static_cast<unsigned>((a->rows + kRowThreads / 32 - 1) / (kRowThreads / 32));
+  auto launch = [&](auto kernel) {
+    kernel<<<grid, kRowThreads, 0, stream>>>(a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->rows, a->channels / 8);
+  };
+  switch (a->out_dtype) {
+    case DMF_INT8_BF16: launch(int8_dequantize_kernel<__nv_bfloat16>); break;
+    case DMF_INT8_FP16: launch(int8_dequantize_kernel<__half>); break;
+    default: launch(int8_dequantize_kernel<float>);
+  }
+  return launched();
+}
+
+}  // namespace
+
+#define DMF_API extern "C" __attribute__((visibility("default")))
+DMF_API int dmf_int8_quantize(const dmf_int8_quantize_args* args) { return run_quantize(args); }
+DMF_API int dmf_int8_rmsnorm(const dmf_int8_rmsnorm_args* args) { return run_rmsnorm(args); }
+DMF_API int dmf_int8_ln_modulate(const dmf_int8_ln_modulate_args* args) { return run_ln_modulate(args); }
+DMF_API int dmf_int8_dequantize(const dmf_int8_dequantize_args* args) { return run_dequantize(args); }

@@ -20,7 +20,7 @@
 
 #include <type_traits>
 
-#include "int8_rows.cuh"
+#include "int8_types.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dmf {

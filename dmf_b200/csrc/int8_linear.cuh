@@ -8,7 +8,7 @@
 
 #include <stdint.h>
 
-#include "int8_rows.cuh"
+#include "int8_types.cuh"
 
 namespace dmf {
 

@@ -1,13 +1,21 @@
 // Rows in 8 bits (include/dmf_int8.h): quantisation behind an activation, RMS norm and LayerNorm-modulate with the
 // residual's addition in front and int8 rows with a scale each behind them, and back to 16 or 32 bits.
 //
-// Any width and alignment: one block per row, the row's values computed again from global memory in every pass (statistics,
-// maximum, output).  Sums and the arithmetic are fp32.
+// HBM-bound: every tensor is read and written once, the row stays in registers between the statistics, the maximum and the
+// output.  int8_row_warp_kernel has a warp per row and the per-channel vectors in shared memory (many rows of up to 1280
+// channels), int8_row_block_kernel a block per row (few rows, where latency counts, and wide ones); both move 16 bytes at a time.
+// int8_row_any_kernel takes what these do not: odd widths, strides and alignments, mixed 16-bit types, rows beyond 16384
+// channels.  Sums and the arithmetic are fp32.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <type_traits>
+
+#include "int8_types.cuh"
+#include "vec8.cuh"
 
 namespace dmf {
 
@@ -21,7 +29,8 @@ struct Int8RowParams {
   int8_t* q;
   float* row_scale;
   int64_t x_sb, x_sl, add_sb, add_sl, sum_sb, sum_sl, gate_sb, shift_sb, scale_sb, q_stride;
-  int seqlen, channels;
+  int64_t rows;
+  int seqlen, channels, batch;
   int x_dtype, add_dtype, sum_dtype, mod_dtype;   // mod: weight / gate, shift, scale
   int act;
   float eps;
@@ -29,17 +38,6 @@ struct Int8RowParams {
 
 constexpr int kRowThreads = 256;
 constexpr float kRowTiny = 7.52316384526264e-37f;   // 2^-120: below it a row counts as zeros (127 / a stays finite)
-
-__device__ __forceinline__ float row_load(const void* p, int dtype, int64_t i) {
-  if (dtype == 0) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  if (dtype == 1) return __half2float(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
-__device__ __forceinline__ void row_store(void* p, int dtype, int64_t i, float v) {
-  if (dtype == 0) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else if (dtype == 1) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<float*>(p)[i] = v;
-}
 
 // GELU in its tanh form, 0.5 x (1 + tanh u) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3); SiLU x / (1 + exp(-x))
 __device__ __forceinline__ float row_act(float x, int act) {
@@ -53,26 +51,34 @@ __device__ __forceinline__ float row_act(float x, int act) {
 struct RowScale {
   float scale, inverse;
 };
+__device__ __forceinline__ float row_warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
 __device__ __forceinline__ RowScale row_scale_of(uint32_t bits) {
   const float a = __uint_as_float(bits);
   if (bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
   if (a < kRowTiny) return {0.f, 0.f};
   return {__fdiv_rn(a, 127.f), __fdiv_rn(127.f, a)};
 }
-__device__ __forceinline__ int row_quantize(float y, const RowScale& s) {
-  return s.inverse == 0.f ? 0 : __float2int_rn(y * s.inverse);
+// The nearest integer, ties to even, in the low byte of the result: adding 1.5 * 2^23 leaves it in the low mantissa bits.  (The
+// conversion instruction shares its unit with the exponentials, at an eighth of the rate of an addition.)
+__device__ __forceinline__ uint32_t row_quantize(float y, const RowScale& s) {
+  return s.inverse == 0.f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(y, s.inverse), 12582912.f));
+}
+__device__ __forceinline__ uint32_t row_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// sums and maxima over the block, returned to every thread
+// sums and maxima over the block, returned to every thread; red: a word per warp
 __device__ __forceinline__ float row_block_sum(float v, float* red) {
-#pragma unroll
-  for (int d = 16; d >= 1; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  v = row_warp_sum(v);
   __syncthreads();  // red is free
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0.f;
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) v += red[w];
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v += red[w];
   return v;
 }
 __device__ __forceinline__ uint32_t row_block_max(uint32_t v, float* red) {
@@ -81,9 +87,221 @@ __device__ __forceinline__ uint32_t row_block_max(uint32_t v, float* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(v);
   __syncthreads();
   v = 0u;
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w) v = max(v, __float_as_uint(red[w]));
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v = max(v, __float_as_uint(red[w]));
   return v;
+}
+
+// Coherent, unlike ld_nc_v4: the sum may be written where its first term was read.
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// Eight consecutive elements as they lie in memory: one 16-byte load of a 16-bit type, two of fp32.
+template <typename T>
+struct Raw8 {
+  uint4 a;
+  __device__ __forceinline__ void load(const void* p, int64_t i) { a = ld_stream_v4(static_cast<const T*>(p) + i); }
+  __device__ __forceinline__ void get(float (&f)[8]) const { unpack8<T>(a, f); }
+  __device__ __forceinline__ static void put(void* p, int64_t i, const float (&f)[8]) { store8(static_cast<T*>(p) + i, f); }
+};
+template <>
+struct Raw8<float> {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    a = ld_stream_v4(static_cast<const float*>(p) + i);
+    b = ld_stream_v4(static_cast<const float*>(p) + i + 4);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
+  }
+  __device__ __forceinline__ static void put(void* p, int64_t i, const float (&f)[8]) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+    d[0] = make_float4(f[0], f[1], f[2], f[3]);
+    d[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+};
+
+// eight channels of a per-channel vector whose type the launch knows
+__device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, float (&f)[8]) {
+  if (dtype == 0) unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + i), f);
+  else if (dtype == 1) unpack8<__half>(*reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + i), f);
+  else {
+    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 a = s[0], b = s[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+}
+
+template <int kAct>
+__device__ __forceinline__ void row_act8(float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = row_act(f[i], kAct);
+}
+
+// A row in registers, thread `t` of `threads` holding eights t, t + threads, ...: the same steps for both kernels.
+//   sum_up, max_up: over the row's threads;  vec(which, c, f): eight channels of 0 gate, 1 weight or 1 + scale, 2 shift
+template <int kOp, typename TX, typename TA, int NV, typename SumUp, typename MaxUp, typename Vec>
+__device__ __forceinline__ void row_in_registers(const Int8RowParams& p, int64_t row, int64_t x0, int64_t add0, int64_t sum0, int t, int threads,
+                                                 SumUp&& sum_up, MaxUp&& max_up, Vec&& vec) {
+  constexpr bool kAdd = !std::is_void<TA>::value;
+  using TAdd = typename std::conditional<kAdd, TA, float>::type;
+  using TSum = typename std::conditional<kOp == kRowLn, TX, TAdd>::type;
+  const int eights = p.channels >> 3;
+  Raw8<TX> rx[NV];
+  Raw8<TAdd> ra[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (t + k * threads < eights) {
+      rx[k].load(p.x, x0 + 8 * (t + k * threads));
+      if constexpr (kAdd) ra[k].load(p.add, add0 + 8 * (t + k * threads));
+    }
+  float z[NV][8];
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (t + k * threads < eights) {
+      rx[k].get(z[k]);
+      if constexpr (kAdd) {
+        float a[8];
+        ra[k].get(a);
+        if constexpr (kOp == kRowRms) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[k][i] += a[i];
+        } else {
+          float g[8];
+          vec(0, 8 * (t + k * threads), g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[k][i] = fmaf(g[i], a[i], z[k][i]);
+        }
+        Raw8<TSum>::put(p.sum, sum0 + 8 * (t + k * threads), z[k]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[k][i] = 0.f;
+    }
+  }
+  if constexpr (kOp == kRowQuantize) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (p.act == 1) row_act8<1>(z[k]);
+      else if (p.act == 2) row_act8<2>(z[k]);
+    }
+  } else {
+    const float inv_c = 1.f / static_cast<float>(p.channels);
+    if constexpr (kOp == kRowLn) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += z[k][i];
+      const float mean = sum_up(s) * inv_c;
+      s = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (t + k * threads < eights)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[k][i] -= mean;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(z[k][i], z[k][i], s);
+    const float r = rsqrtf(sum_up(s) * inv_c + p.eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (t + k * threads < eights) {
+        const int c = 8 * (t + k * threads);
+        float w[8], b[8];
+        vec(1, c, w);
+        if constexpr (kOp == kRowLn) vec(2, c, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[k][i] = kOp == kRowLn ? fmaf(z[k][i] * r, w[i], b[i]) : z[k][i] * r * w[i];
+      }
+  }
+  uint32_t bits = 0u;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(fabsf(z[k][i])));
+  const RowScale rs = row_scale_of(max_up(bits));
+  int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (t + k * threads < eights) {
+      uint32_t u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = row_quantize(z[k][i], rs);
+      *reinterpret_cast<uint2*>(q + 8 * (t + k * threads)) = make_uint2(row_pack4(u[0], u[1], u[2], u[3]), row_pack4(u[4], u[5], u[6], u[7]));
+    }
+  if (t == 0) p.row_scale[row] = rs.scale;
+}
+
+// A warp per row.  grid (blocks over the rows of a sample, samples): block x owns rows [x * rows_per_block, ...) of sample y, so
+// that the sample's vectors are staged once per block, as fp32.  (RMS norm and quantisation see all rows as one sample.)
+template <int kOp, typename TX, typename TA, int NV>
+__global__ void __launch_bounds__(kRowThreads) int8_row_warp_kernel(const Int8RowParams p, int rows_per_block) {
+  constexpr int kVecs = kOp == kRowQuantize ? 0 : (kOp == kRowRms ? 1 : (std::is_void<TA>::value ? 2 : 3));
+  __shared__ __align__(16) float s_vec[kVecs > 0 ? kVecs * NV * 256 : 4];   // [weight or 1 + scale | shift | gate]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t b0 = blockIdx.y;
+  if constexpr (kVecs > 0) {
+    for (int c = 8 * threadIdx.x; c < p.channels; c += 8 * kRowThreads) {
+      float f[8];
+      auto stage = [&](int which, const void* src, int64_t at, float plus) {
+        row_vec8(src, p.mod_dtype, at + c, f);
+        float4* d = reinterpret_cast<float4*>(s_vec + which * NV * 256 + c);
+        d[0] = make_float4(f[0] + plus, f[1] + plus, f[2] + plus, f[3] + plus);
+        d[1] = make_float4(f[4] + plus, f[5] + plus, f[6] + plus, f[7] + plus);
+      };
+      if constexpr (kOp == kRowRms) {
+        stage(0, p.weight, 0, 0.f);
+      } else {
+        stage(0, p.scale, b0 * p.scale_sb, 1.f);
+        stage(1, p.shift, b0 * p.shift_sb, 0.f);
+        if constexpr (kVecs == 3) stage(2, p.gate, b0 * p.gate_sb, 0.f);
+      }
+    }
+    __syncthreads();
+  }
+  auto vec = [&](int which, int c, float (&f)[8]) {
+    const float4* v = reinterpret_cast<const float4*>(s_vec + (which == 0 ? 2 : which - 1) * NV * 256 + c);
+    const float4 a = v[0], b = v[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  };
+  const int64_t per_sample = kOp == kRowLn ? p.seqlen : p.rows;
+  const int64_t l0 = static_cast<int64_t>(blockIdx.x) * rows_per_block, l1 = min(per_sample, l0 + rows_per_block);
+  for (int64_t l = l0 + warp; l < l1; l += kRowThreads / 32) {
+    const int64_t row = b0 * per_sample + l;
+    const int64_t b = kOp == kRowLn ? b0 : row / p.seqlen, i = kOp == kRowLn ? l : row % p.seqlen;
+    row_in_registers<kOp, TX, TA, NV>(
+        p, row, b * p.x_sb + i * p.x_sl, b * p.add_sb + i * p.add_sl, b * p.sum_sb + i * p.sum_sl, lane, 32,
+        [](float v) { return row_warp_sum(v); }, [](uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }, vec);
+  }
+}
+
+// A block per row, the vectors from global memory.
+constexpr int block_row_threads(int nv) { return nv == 1 ? 1024 : 512; }   // most threads of a block
+template <int kOp, typename TX, typename TA, int NV>
+__global__ void __launch_bounds__(block_row_threads(NV)) int8_row_block_kernel(const Int8RowParams p) {
+  __shared__ float red[32];
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / p.seqlen, l = row % p.seqlen;
+  row_in_registers<kOp, TX, TA, NV>(
+      p, row, b * p.x_sb + l * p.x_sl, b * p.add_sb + l * p.add_sl, b * p.sum_sb + l * p.sum_sl, threadIdx.x, blockDim.x,
+      [&](float v) { return row_block_sum(v, red); }, [&](uint32_t v) { return row_block_max(v, red); },
+      [&](int which, int c, float (&f)[8]) {
+        if (which == 0) row_vec8(p.gate, p.mod_dtype, b * p.gate_sb + c, f);
+        else if (which == 2) row_vec8(p.shift, p.mod_dtype, b * p.shift_sb + c, f);
+        else if (kOp == kRowRms) row_vec8(p.weight, p.mod_dtype, c, f);
+        else {
+          row_vec8(p.scale, p.mod_dtype, b * p.scale_sb + c, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] += 1.f;
+        }
+      });
 }
 
 template <int kOp>
@@ -129,9 +347,28 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
     const float z = z_at(c);
     if (kOp != kRowQuantize && p.sum != nullptr) row_store(p.sum, p.sum_dtype, sum0 + c, z);
-    p.q[row * p.q_stride + c] = static_cast<int8_t>(row_quantize(y_of(z, c), s));
+    p.q[row * p.q_stride + c] = static_cast<int8_t>(row_quantize(y_of(z, c), s) & 0xffu);
   }
   if (threadIdx.x == 0) p.row_scale[row] = s.scale;
+}
+
+// A warp per row, eight elements per lane and step.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int64_t rows, int eights) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float s = scale[row];
+  const uint2* src = reinterpret_cast<const uint2*>(q + row * q_stride);
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int k = lane; k < eights; k += 32) {
+    const uint2 v = src[k];
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)))) * s;
+    Raw8<T>::put(out, row * out_stride + 8 * k, f);
+  }
 }
 
 __global__ void __launch_bounds__(kRowThreads)
