@@ -39,15 +39,31 @@ struct Int8RowParams {
 constexpr int kRowThreads = 256;
 constexpr float kRowTiny = 7.52316384526264e-37f;   // 2^-120: below it a row counts as zeros (127 / a stays finite)
 
-// GELU in its tanh form, 0.5 x (1 + tanh u) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3); SiLU x / (1 + exp(-x))
-__device__ __forceinline__ float row_act(float x, int act) {
-  if (act == 0) return x;
-  const float t = act == 1 ? 2.f * 0.7978845608028654f * fmaf(0.044715f * x, x * x, x) : x;
-  return __fdividef(x, 1.f + __expf(-t));
+__device__ __forceinline__ float row_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// SiLU x / (1 + exp(-x)); GELU in its tanh form, 0.5 x (1 + tanh u) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// Both as x / (1 + 2^v): where 2^v overflows the result is 0 (of -infinity NaN, as the formulas have it).
+template <int kAct>
+__device__ __forceinline__ float row_act(float x) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if constexpr (kAct == 0) return x;
+  constexpr float c1 = -2.f * 0.7978845608028654f * kLog2e;
+  const float v = kAct == 1 ? x * fmaf(c1 * 0.044715f, x * x, c1) : -kLog2e * x;
+  return x * row_rcp(1.f + fast_exp2(v));
 }
 
-// What a row's maximum makes of it.  `bits`: max of |y| as unsigned bit patterns, which order like the values with infinity
-// and then NaN behind them, so a NaN is not lost as it is in fmaxf.
+// max(m, |a|, |b|), NaN if one of them is
+__device__ __forceinline__ float row_max3(float m, float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return d;
+}
+
+// What a row's maximum makes of it.  `bits`: of the maximum of |y|; as unsigned numbers bit patterns order like the values, with
+// infinity and then NaN behind them.
 struct RowScale {
   float scale, inverse;
 };
@@ -63,9 +79,9 @@ __device__ __forceinline__ RowScale row_scale_of(uint32_t bits) {
   return {__fdiv_rn(a, 127.f), __fdiv_rn(127.f, a)};
 }
 // The nearest integer, ties to even, in the low byte of the result: adding 1.5 * 2^23 leaves it in the low mantissa bits.  (The
-// conversion instruction shares its unit with the exponentials, at an eighth of the rate of an addition.)
-__device__ __forceinline__ uint32_t row_quantize(float y, const RowScale& s) {
-  return s.inverse == 0.f ? 0u : __float_as_uint(__fadd_rn(__fmul_rn(y, s.inverse), 12582912.f));
+// conversion instruction shares its unit with the exponentials, at an eighth of the rate of an addition.)  Not for inverse = 0.
+__device__ __forceinline__ uint32_t row_quantize(float y, float inverse) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(y, inverse), 12582912.f));
 }
 __device__ __forceinline__ uint32_t row_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
@@ -139,7 +155,7 @@ __device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, fl
 template <int kAct>
 __device__ __forceinline__ void row_act8(float (&f)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = row_act(f[i], kAct);
+  for (int i = 0; i < 8; ++i) f[i] = row_act<kAct>(f[i]);
 }
 
 // A row in registers, thread `t` of `threads` holding eights t, t + threads, ...: the same steps for both kernels.
@@ -221,20 +237,25 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, int64_t
         for (int i = 0; i < 8; ++i) z[k][i] = kOp == kRowLn ? fmaf(z[k][i] * r, w[i], b[i]) : z[k][i] * r * w[i];
       }
   }
-  uint32_t bits = 0u;
+  float top = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(fabsf(z[k][i])));
-  const RowScale rs = row_scale_of(max_up(bits));
+    for (int i = 0; i < 8; i += 2) top = row_max3(top, z[k][i], z[k][i + 1]);
+  const RowScale rs = row_scale_of(max_up(__float_as_uint(top)));
   int8_t* q = p.q + row * p.q_stride;
+  const bool zeros = rs.inverse == 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
     if (t + k * threads < eights) {
-      uint32_t u[8];
+      uint2 out = make_uint2(0u, 0u);
+      if (!zeros) {
+        uint32_t u[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = row_quantize(z[k][i], rs);
-      *reinterpret_cast<uint2*>(q + 8 * (t + k * threads)) = make_uint2(row_pack4(u[0], u[1], u[2], u[3]), row_pack4(u[4], u[5], u[6], u[7]));
+        for (int i = 0; i < 8; ++i) u[i] = row_quantize(z[k][i], rs.inverse);
+        out = make_uint2(row_pack4(u[0], u[1], u[2], u[3]), row_pack4(u[4], u[5], u[6], u[7]));
+      }
+      *reinterpret_cast<uint2*>(q + 8 * (t + k * threads)) = out;
     }
   if (t == 0) p.row_scale[row] = rs.scale;
 }
@@ -313,7 +334,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   const float inv_c = 1.f / static_cast<float>(p.channels);
   auto z_at = [&](int c) -> float {
     const float x = row_load(p.x, p.x_dtype, x0 + c);
-    if constexpr (kOp == kRowQuantize) return row_act(x, p.act);
+    if constexpr (kOp == kRowQuantize) return p.act == 1 ? row_act<1>(x) : (p.act == 2 ? row_act<2>(x) : x);
     if (p.add == nullptr) return x;
     const float a = row_load(p.add, p.add_dtype, add0 + c);
     if constexpr (kOp == kRowRms) return a + x;
@@ -347,7 +368,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
     const float z = z_at(c);
     if (kOp != kRowQuantize && p.sum != nullptr) row_store(p.sum, p.sum_dtype, sum0 + c, z);
-    p.q[row * p.q_stride + c] = static_cast<int8_t>(row_quantize(y_of(z, c), s) & 0xffu);
+    p.q[row * p.q_stride + c] = static_cast<int8_t>(s.inverse == 0.f ? 0u : row_quantize(y_of(z, c), s.inverse) & 0xffu);
   }
   if (threadIdx.x == 0) p.row_scale[row] = s.scale;
 }
@@ -364,9 +385,11 @@ int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, vo
 #pragma unroll 4
   for (int k = lane; k < eights; k += 32) {
     const uint2 v = src[k];
+    // q + 128 in the low mantissa bits of 2^23 is 2^23 + 128 + q, exactly; the conversion instruction is slow
+    const uint32_t u[2] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u};
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)))) * s;
+    for (int i = 0; i < 8; ++i) f[i] = (__uint_as_float(__byte_perm(u[i >> 2], 0x4b000000u, 0x7540 + (i & 3))) - 8388736.f) * s;
     Raw8<T>::put(out, row * out_stride + 8 * k, f);
   }
 }
