@@ -1,8 +1,10 @@
 // C ABI of inference in 8-bit integers (include/dmf_int8.h), rows: quantisation, norms with 8-bit results, and the way back.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
+#include "attn_launch.h"
 #include "dmf_attn.h"
 #include "dmf_int8.h"
 #include "int8_launch.h"
@@ -46,66 +48,82 @@ bool reads_vectors(const Int8RowParams& p, int op) {
   return ok;
 }
 
-constexpr int kWarpRowEights = 160;    // a warp's registers hold rows of up to 5 x 32 eights
-
-// A warp per row where that fills the SMs with warps; the LayerNorm form, whose blocks stay within a sample, also needs a few
-// rows of a sample per block.
-bool warp_per_row(const Int8RowParams& p, int op, int sms) {
-  return p.channels / 8 <= kWarpRowEights && p.rows >= 8ll * sms && (op != kRowLn || (p.seqlen >= 8 && p.batch <= 65535));
+// Blocks of a kernel that an SM holds.
+int blocks_per_sm(int registers, int threads, int smem) {
+  const int by_registers = 65536 / ((registers + 7) / 8 * 8 * threads), by_threads = 2048 / threads, by_smem = smem > 0 ? 227 * 1024 / (smem + 1280) : 32;
+  int blocks = by_registers < by_threads ? by_registers : by_threads;
+  if (by_smem < blocks) blocks = by_smem;
+  return blocks > 1 ? blocks : 1;
 }
 
-// Rows of one block of the warp kernel: the vectors are staged once per block, so many, as long as every SM has a few blocks.
-int rows_per_block(int64_t samples, int64_t rows_of_sample, int sms) {
-  for (int rpb = 32; rpb > 8; rpb /= 2)
-    if (samples * ((rows_of_sample + rpb - 1) / rpb) >= 4ll * sms) return rpb;
-  return 8;
+constexpr int kWarpRowEights = 160;            // a warp's registers hold rows of up to 5 x 32 eights
+constexpr int kMaxEights = 4 * kGroupThreads;  // a block's: 4 per thread
+
+// The loop over rows where that fills the SMs; the LayerNorm form, whose blocks stay within a sample, also wants a few rows of a
+// sample per block.
+bool many_rows(const Int8RowParams& p, int op, int sms) {
+  if (p.channels / 8 > 1024) return true;      // more than the threads of a block per row
+  return p.rows >= 8ll * sms && (op != kRowLn || (p.seqlen >= 8 && p.batch <= 65535));
+}
+
+template <int kOp, typename TX, typename TA, int NV, bool kWarp>
+int launch_group(const Int8RowParams& p, int threads, int sms, cudaStream_t stream) {
+  static bool allowed[64];
+  const auto kernel = int8_row_group_kernel<kOp, TX, TA, NV, kWarp>;
+  const int smem = kRowVectors<kOp, TA> * p.channels * 4;
+  if (smem > 48 * 1024 && !allow_smem(kernel, kRowVectors<kOp, TA> * kMaxEights * 32, allowed)) return DMF_ATTN_ERR_LAUNCH;
+  static std::atomic<int> registers{0};
+  if (registers.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return DMF_ATTN_ERR_LAUNCH;
+    }
+    registers.store(attr.numRegs, std::memory_order_relaxed);
+  }
+  // one wave: as many blocks as the SMs hold at a time, cut at the samples' ends
+  const int64_t samples = kOp == kRowLn ? p.batch : 1, per_sample = kOp == kRowLn ? p.seqlen : p.rows, unit = kWarp ? kRowThreads / 32 : 1;
+  const int64_t resident = static_cast<int64_t>(sms) * blocks_per_sm(registers.load(std::memory_order_relaxed), threads, smem);
+  const int64_t splits = resident / samples > 1 ? resident / samples : 1;
+  const int64_t units = (per_sample + unit - 1) / unit;
+  const int rpb = static_cast<int>((units + splits - 1) / splits * unit);
+  const dim3 grid(static_cast<unsigned>((per_sample + rpb - 1) / rpb), static_cast<unsigned>(samples));
+  kernel<<<grid, threads, smem, stream>>>(p, rpb);
+  return launched();
 }
 
 template <int kOp, typename TX, typename TA>
-void launch_vectors(const Int8RowParams& p, int sms, cudaStream_t stream) {
-  const int eights = p.channels / 8;
-  if (warp_per_row(p, kOp, sms)) {
-    const int64_t samples = kOp == kRowLn ? p.batch : 1, per_sample = kOp == kRowLn ? p.seqlen : p.rows;
-    const int rpb = kOp == kRowQuantize ? kRowThreads / 32 : rows_per_block(samples, per_sample, sms);
-    const dim3 grid(static_cast<unsigned>((per_sample + rpb - 1) / rpb), static_cast<unsigned>(samples));
-    if (eights <= 64) int8_row_warp_kernel<kOp, TX, TA, 2><<<grid, kRowThreads, 0, stream>>>(p, rpb);
-    else int8_row_warp_kernel<kOp, TX, TA, 5><<<grid, kRowThreads, 0, stream>>>(p, rpb);
-    return;
+int launch_vectors(const Int8RowParams& p, int sms, cudaStream_t stream) {
+  const int eights = p.channels / 8, wide = ((eights + 3) / 4 + 31) / 32 * 32;   // threads, four eights each
+  const unsigned rows = static_cast<unsigned>(p.rows);
+  if (!many_rows(p, kOp, sms)) {
+    int8_row_block_kernel<kOp, TX, TA, 1><<<rows, (eights + 31) / 32 * 32, 0, stream>>>(p);
+    return launched();
   }
-  // one eight per thread for few rows, four for many: fewer threads per row then leave room for more rows on an SM
-  const bool one = eights <= 1024 && p.rows < 4ll * sms;
-  const int per = one ? 1 : 4, threads = ((eights + per - 1) / per + 31) / 32 * 32;
-  const unsigned grid = static_cast<unsigned>(p.rows);
-  if (one) int8_row_block_kernel<kOp, TX, TA, 1><<<grid, threads, 0, stream>>>(p);
-  else int8_row_block_kernel<kOp, TX, TA, 4><<<grid, threads, 0, stream>>>(p);
+  if (eights <= 64) return launch_group<kOp, TX, TA, 2, true>(p, kRowThreads, sms, stream);
+  if (eights <= kWarpRowEights) return launch_group<kOp, TX, TA, 5, true>(p, kRowThreads, sms, stream);
+  if constexpr (kOp == kRowLn) return launch_group<kOp, TX, TA, 4, false>(p, wide, sms, stream);
+  int8_row_block_kernel<kOp, TX, TA, 4><<<rows, wide, 0, stream>>>(p);
+  return launched();
 }
 
-// false: a pair of types without a kernel of its own
+constexpr int kNoKernel = -1;   // of launch_types: a pair of types without a kernel of its own
+
 template <int kOp, typename TX>
-bool launch_types(const Int8RowParams& p, int sms, cudaStream_t stream) {
+int launch_types(const Int8RowParams& p, int sms, cudaStream_t stream) {
   if constexpr (kOp != kRowQuantize) {
     if (p.add != nullptr) {
       constexpr bool kF32 = std::is_same<TX, float>::value;
-      if (p.add_dtype == DMF_INT8_F32) {
-        launch_vectors<kOp, TX, float>(p, sms, stream);
-        return true;
-      }
+      if (p.add_dtype == DMF_INT8_F32) return launch_vectors<kOp, TX, float>(p, sms, stream);
       if (p.add_dtype == DMF_INT8_BF16) {
-        if constexpr (kF32 || std::is_same<TX, __nv_bfloat16>::value) {
-          launch_vectors<kOp, TX, __nv_bfloat16>(p, sms, stream);
-          return true;
-        }
+        if constexpr (kF32 || std::is_same<TX, __nv_bfloat16>::value) return launch_vectors<kOp, TX, __nv_bfloat16>(p, sms, stream);
       } else {
-        if constexpr (kF32 || std::is_same<TX, __half>::value) {
-          launch_vectors<kOp, TX, __half>(p, sms, stream);
-          return true;
-        }
+        if constexpr (kF32 || std::is_same<TX, __half>::value) return launch_vectors<kOp, TX, __half>(p, sms, stream);
       }
-      return false;
+      return kNoKernel;
     }
   }
-  launch_vectors<kOp, TX, void>(p, sms, stream);
-  return true;
+  return launch_vectors<kOp, TX, void>(p, sms, stream);
 }
 
 template <int kOp>
@@ -113,15 +131,16 @@ int launch_rows(const Int8RowParams& p, cudaStream_t stream) {
   int sms = 0, st = sm_count_of_current_device(&sms);
   if (st != DMF_ATTN_OK) return st;
   if (p.rows == 0) return DMF_ATTN_OK;
-  bool done = false;
-  if (reads_vectors(p, kOp) && p.channels / 8 <= 4 * block_row_threads(4)) {
+  // (65535: samples are a grid dimension of the kernel that a LayerNorm of more than 8192 channels takes whatever its rows)
+  if (reads_vectors(p, kOp) && p.channels / 8 <= kMaxEights && (kOp != kRowLn || p.channels <= 8192 || p.batch <= 65535)) {
     switch (p.x_dtype) {
-      case DMF_INT8_BF16: done = launch_types<kOp, __nv_bfloat16>(p, sms, stream); break;
-      case DMF_INT8_FP16: done = launch_types<kOp, __half>(p, sms, stream); break;
-      default: done = launch_types<kOp, float>(p, sms, stream);
+      case DMF_INT8_BF16: st = launch_types<kOp, __nv_bfloat16>(p, sms, stream); break;
+      case DMF_INT8_FP16: st = launch_types<kOp, __half>(p, sms, stream); break;
+      default: st = launch_types<kOp, float>(p, sms, stream);
     }
+    if (st != kNoKernel) return st;
   }
-  if (!done) int8_row_any_kernel<kOp><<<static_cast<unsigned>(p.rows), kRowThreads, 0, stream>>>(p);
+  int8_row_any_kernel<kOp><<<static_cast<unsigned>(p.rows), kRowThreads, 0, stream>>>(p);
   return launched();
 }
 
@@ -227,9 +246,12 @@ int run_dequantize(const dmf_int8_dequantize_args* a) {
         a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->out_dtype, a->channels);
     return launched();
   }
-  const unsigned grid = static_cast<unsigned>((a->rows + kRowThreads / 32 - 1) / (kRowThreads / 32));
+  const int eights = a->channels / 8, pieces = (eights + kDequantizeEights - 1) / kDequantizeEights;
+  const int64_t blocks = (a->rows * pieces + kRowThreads / 32 - 1) / (kRowThreads / 32);
+  if (blocks > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;
   auto launch = [&](auto kernel) {
-    kernel<<<grid, kRowThreads, 0, stream>>>(a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->rows, a->channels / 8);
+    kernel<<<static_cast<unsigned>(blocks), kRowThreads, 0, stream>>>(a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->rows,
+                                                                      eights, pieces);
   };
   switch (a->out_dtype) {
     case DMF_INT8_BF16: launch(int8_dequantize_kernel<__nv_bfloat16>); break;

@@ -2,8 +2,11 @@
 // residual's addition in front and int8 rows with a scale each behind them, and back to 16 or 32 bits.
 //
 // HBM-bound: every tensor is read and written once, the row stays in registers between the statistics, the maximum and the
-// output.  int8_row_warp_kernel has a warp per row and the per-channel vectors in shared memory (many rows of up to 1280
-// channels), int8_row_block_kernel a block per row (few rows, where latency counts, and wide ones); both move 16 bytes at a time.
+// output.  int8_row_group_kernel has a warp (rows of up to 1280 channels) or a block (wider ones, LayerNorm) take row after row,
+// the loads of the next one under way while it works on the present one, and the per-channel vectors in shared memory.
+// int8_row_block_kernel has a block per row: few rows, where latency counts, and wide ones without a sample's vectors, where
+// blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 45 us
+// against 51, with GELU 66 against 78; gated LayerNorm 189 against 133).  Both move 16 bytes at a time.
 // int8_row_any_kernel takes what these do not: odd widths, strides and alignments, mixed 16-bit types, rows beyond 16384
 // channels.  Sums and the arithmetic are fp32.
 #pragma once
@@ -87,23 +90,24 @@ __device__ __forceinline__ uint32_t row_pack4(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// sums and maxima over the block, returned to every thread; red: a word per warp
-__device__ __forceinline__ float row_block_sum(float v, float* red) {
+// Sums and maxima over the block, returned to every thread.  red: two rows of a word per warp, used in turn (`turn` counts), so
+// that one barrier per reduction is enough: a row is written again only behind the barrier that follows its last reading.
+__device__ __forceinline__ float row_block_sum(float v, float (*red)[32], int& turn) {
+  float* r = red[turn++ & 1];
   v = row_warp_sum(v);
-  __syncthreads();  // red is free
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0.f;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v += red[w];
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v += r[w];
   return v;
 }
-__device__ __forceinline__ uint32_t row_block_max(uint32_t v, float* red) {
+__device__ __forceinline__ uint32_t row_block_max(uint32_t v, float (*red)[32], int& turn) {
+  float* r = red[turn++ & 1];
   v = __reduce_max_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(v);
+  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = __uint_as_float(v);
   __syncthreads();
   v = 0u;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v = max(v, __float_as_uint(red[w]));
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v = max(v, __float_as_uint(r[w]));
   return v;
 }
 
@@ -158,32 +162,43 @@ __device__ __forceinline__ void row_act8(float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = row_act<kAct>(f[i]);
 }
 
-// A row in registers, thread `t` of `threads` holding eights t, t + threads, ...: the same steps for both kernels.
-//   sum_up, max_up: over the row's threads;  vec(which, c, f): eight channels of 0 gate, 1 weight or 1 + scale, 2 shift
-template <int kOp, typename TX, typename TA, int NV, typename SumUp, typename MaxUp, typename Vec>
-__device__ __forceinline__ void row_in_registers(const Int8RowParams& p, int64_t row, int64_t x0, int64_t add0, int64_t sum0, int t, int threads,
-                                                 SumUp&& sum_up, MaxUp&& max_up, Vec&& vec) {
-  constexpr bool kAdd = !std::is_void<TA>::value;
+// A row in registers, thread `t` of `threads` holding eights t, t + threads, ...
+template <int kOp, typename TX, typename TA, int NV>
+struct RowLoads {
+  static constexpr bool kAdd = !std::is_void<TA>::value;
   using TAdd = typename std::conditional<kAdd, TA, float>::type;
-  using TSum = typename std::conditional<kOp == kRowLn, TX, TAdd>::type;
-  const int eights = p.channels >> 3;
-  Raw8<TX> rx[NV];
-  Raw8<TAdd> ra[NV];
+  Raw8<TX> x[NV];
+  Raw8<TAdd> add[NV];
+  __device__ __forceinline__ void start(const Int8RowParams& p, int64_t x0, int64_t add0, int t, int threads) {
+    const int eights = p.channels >> 3;
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (t + k * threads < eights) {
-      rx[k].load(p.x, x0 + 8 * (t + k * threads));
-      if constexpr (kAdd) ra[k].load(p.add, add0 + 8 * (t + k * threads));
-    }
+    for (int k = 0; k < NV; ++k)
+      if (t + k * threads < eights) {
+        x[k].load(p.x, x0 + 8 * (t + k * threads));
+        if constexpr (kAdd) add[k].load(p.add, add0 + 8 * (t + k * threads));
+      }
+  }
+};
+
+// What both kernels do with a loaded row.
+//   load_next: called once the loads are in z;  sum_up, max_up: over the row's threads
+//   vec(which, c, f): eight channels of 0 gate, 1 weight or 1 + scale, 2 shift
+template <int kOp, typename TX, typename TA, int NV, typename Next, typename SumUp, typename MaxUp, typename Vec>
+__device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoads<kOp, TX, TA, NV>& loads, int64_t row, int64_t sum0, int t,
+                                                 int threads, Next&& load_next, SumUp&& sum_up, MaxUp&& max_up, Vec&& vec) {
+  using Loads = RowLoads<kOp, TX, TA, NV>;
+  constexpr bool kAdd = Loads::kAdd;
+  using TSum = typename std::conditional<kOp == kRowLn, TX, typename Loads::TAdd>::type;
+  const int eights = p.channels >> 3;
   float z[NV][8];
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     if (t + k * threads < eights) {
-      rx[k].get(z[k]);
+      loads.x[k].get(z[k]);
       if constexpr (kAdd) {
         float a[8];
-        ra[k].get(a);
+        loads.add[k].get(a);
         if constexpr (kOp == kRowRms) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) z[k][i] += a[i];
@@ -200,6 +215,7 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, int64_t
       for (int i = 0; i < 8; ++i) z[k][i] = 0.f;
     }
   }
+  load_next();
   if constexpr (kOp == kRowQuantize) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -260,20 +276,25 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, int64_t
   if (t == 0) p.row_scale[row] = rs.scale;
 }
 
-// A warp per row.  grid (blocks over the rows of a sample, samples): block x owns rows [x * rows_per_block, ...) of sample y, so
-// that the sample's vectors are staged once per block, as fp32.  (RMS norm and quantisation see all rows as one sample.)
-template <int kOp, typename TX, typename TA, int NV>
-__global__ void __launch_bounds__(kRowThreads) int8_row_warp_kernel(const Int8RowParams p, int rows_per_block) {
-  constexpr int kVecs = kOp == kRowQuantize ? 0 : (kOp == kRowRms ? 1 : (std::is_void<TA>::value ? 2 : 3));
-  __shared__ __align__(16) float s_vec[kVecs > 0 ? kVecs * NV * 256 : 4];   // [weight or 1 + scale | shift | gate]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Many rows.  kWarp: a warp per row, eight rows of a block at a time; else the whole block on one row.  grid (blocks over the rows
+// of a sample, samples): block x owns rows [x * rows_per_block, ...) of sample y, so that the sample's vectors are staged once per
+// block, as fp32.  (RMS norm and quantisation see all rows as one sample.)
+constexpr int kGroupThreads = 512;      // most threads of a block that works on one row
+template <int kOp, typename TA>
+constexpr int kRowVectors = kOp == kRowQuantize ? 0 : (kOp == kRowRms ? 1 : (std::is_void<TA>::value ? 2 : 3));
+
+template <int kOp, typename TX, typename TA, int NV, bool kWarp>
+__global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_group_kernel(const Int8RowParams p, int rows_per_block) {
+  extern __shared__ __align__(16) float s_vec[];   // kRowVectors x channels: [weight or 1 + scale | shift | gate]
+  __shared__ float red[2][32];
+  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, threads = kWarp ? 32 : blockDim.x;
   const int64_t b0 = blockIdx.y;
-  if constexpr (kVecs > 0) {
-    for (int c = 8 * threadIdx.x; c < p.channels; c += 8 * kRowThreads) {
+  if constexpr (kRowVectors<kOp, TA> > 0) {
+    for (int c = 8 * threadIdx.x; c < p.channels; c += 8 * blockDim.x) {
       float f[8];
       auto stage = [&](int which, const void* src, int64_t at, float plus) {
         row_vec8(src, p.mod_dtype, at + c, f);
-        float4* d = reinterpret_cast<float4*>(s_vec + which * NV * 256 + c);
+        float4* d = reinterpret_cast<float4*>(s_vec + which * p.channels + c);
         d[0] = make_float4(f[0] + plus, f[1] + plus, f[2] + plus, f[3] + plus);
         d[1] = make_float4(f[4] + plus, f[5] + plus, f[6] + plus, f[7] + plus);
       };
@@ -282,37 +303,51 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_warp_kernel(const Int8Ro
       } else {
         stage(0, p.scale, b0 * p.scale_sb, 1.f);
         stage(1, p.shift, b0 * p.shift_sb, 0.f);
-        if constexpr (kVecs == 3) stage(2, p.gate, b0 * p.gate_sb, 0.f);
+        if constexpr (kRowVectors<kOp, TA> == 3) stage(2, p.gate, b0 * p.gate_sb, 0.f);
       }
     }
     __syncthreads();
   }
   auto vec = [&](int which, int c, float (&f)[8]) {
-    const float4* v = reinterpret_cast<const float4*>(s_vec + (which == 0 ? 2 : which - 1) * NV * 256 + c);
+    const float4* v = reinterpret_cast<const float4*>(s_vec + (which == 0 ? 2 : which - 1) * p.channels + c);
     const float4 a = v[0], b = v[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
   };
   const int64_t per_sample = kOp == kRowLn ? p.seqlen : p.rows;
   const int64_t l0 = static_cast<int64_t>(blockIdx.x) * rows_per_block, l1 = min(per_sample, l0 + rows_per_block);
-  for (int64_t l = l0 + warp; l < l1; l += kRowThreads / 32) {
-    const int64_t row = b0 * per_sample + l;
-    const int64_t b = kOp == kRowLn ? b0 : row / p.seqlen, i = kOp == kRowLn ? l : row % p.seqlen;
+  constexpr int kStep = kWarp ? kRowThreads / 32 : 1;
+  RowLoads<kOp, TX, TA, NV> loads;
+  auto start = [&](int64_t l) {
+    const int64_t b = kOp == kRowLn ? b0 : l / p.seqlen, i = kOp == kRowLn ? l : l % p.seqlen;
+    loads.start(p, b * p.x_sb + i * p.x_sl, b * p.add_sb + i * p.add_sl, t, threads);
+  };
+  int turn = 0;
+  int64_t l = l0 + (kWarp ? threadIdx.x >> 5 : 0);
+  if (l < l1) start(l);
+  for (; l < l1; l += kStep) {
+    const int64_t b = kOp == kRowLn ? b0 : l / p.seqlen, i = kOp == kRowLn ? l : l % p.seqlen;
     row_in_registers<kOp, TX, TA, NV>(
-        p, row, b * p.x_sb + i * p.x_sl, b * p.add_sb + i * p.add_sl, b * p.sum_sb + i * p.sum_sl, lane, 32,
-        [](float v) { return row_warp_sum(v); }, [](uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }, vec);
+        p, loads, b0 * per_sample + l, b * p.sum_sb + i * p.sum_sl, t, threads,
+        [&] {
+          if (l + kStep < l1) start(l + kStep);
+        },
+        [&](float v) { return kWarp ? row_warp_sum(v) : row_block_sum(v, red, turn); },
+        [&](uint32_t v) { return kWarp ? __reduce_max_sync(0xffffffffu, v) : row_block_max(v, red, turn); }, vec);
   }
 }
 
 // A block per row, the vectors from global memory.
-constexpr int block_row_threads(int nv) { return nv == 1 ? 1024 : 512; }   // most threads of a block
 template <int kOp, typename TX, typename TA, int NV>
-__global__ void __launch_bounds__(block_row_threads(NV)) int8_row_block_kernel(const Int8RowParams p) {
-  __shared__ float red[32];
+__global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block_kernel(const Int8RowParams p) {
+  __shared__ float red[2][32];
+  int turn = 0;
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.seqlen, l = row % p.seqlen;
+  RowLoads<kOp, TX, TA, NV> loads;
+  loads.start(p, b * p.x_sb + l * p.x_sl, b * p.add_sb + l * p.add_sl, threadIdx.x, blockDim.x);
   row_in_registers<kOp, TX, TA, NV>(
-      p, row, b * p.x_sb + l * p.x_sl, b * p.add_sb + l * p.add_sl, b * p.sum_sb + l * p.sum_sl, threadIdx.x, blockDim.x,
-      [&](float v) { return row_block_sum(v, red); }, [&](uint32_t v) { return row_block_max(v, red); },
+      p, loads, row, b * p.sum_sb + l * p.sum_sl, threadIdx.x, blockDim.x, [] {}, [&](float v) { return row_block_sum(v, red, turn); },
+      [&](uint32_t v) { return row_block_max(v, red, turn); },
       [&](int which, int c, float (&f)[8]) {
         if (which == 0) row_vec8(p.gate, p.mod_dtype, b * p.gate_sb + c, f);
         else if (which == 2) row_vec8(p.shift, p.mod_dtype, b * p.shift_sb + c, f);
@@ -327,7 +362,8 @@ __global__ void __launch_bounds__(block_row_threads(NV)) int8_row_block_kernel(c
 
 template <int kOp>
 __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8RowParams p) {
-  __shared__ float red[kRowThreads / 32];
+  __shared__ float red[2][32];
+  int turn = 0;
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.seqlen, l = row % p.seqlen;
   const int64_t x0 = b * p.x_sb + l * p.x_sl, add0 = b * p.add_sb + l * p.add_sl, sum0 = b * p.sum_sb + l * p.sum_sl;
@@ -344,7 +380,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   if constexpr (kOp == kRowLn) {
     float s = 0.f;
     for (int c = threadIdx.x; c < p.channels; c += kRowThreads) s += z_at(c);
-    mean = row_block_sum(s, red) * inv_c;
+    mean = row_block_sum(s, red, turn) * inv_c;
   }
   if constexpr (kOp != kRowQuantize) {
     float s = 0.f;
@@ -352,7 +388,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
       const float z = z_at(c) - mean;
       s = fmaf(z, z, s);
     }
-    r = rsqrtf(row_block_sum(s, red) * inv_c + p.eps);
+    r = rsqrtf(row_block_sum(s, red, turn) * inv_c + p.eps);
   }
   auto y_of = [&](float z, int c) -> float {
     if constexpr (kOp == kRowQuantize) return z;
@@ -363,7 +399,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   uint32_t bits = 0u;
   for (int c = threadIdx.x; c < p.channels; c += kRowThreads)
     bits = max(bits, __float_as_uint(fabsf(y_of(z_at(c), c))));
-  const RowScale s = row_scale_of(row_block_max(bits, red));
+  const RowScale s = row_scale_of(row_block_max(bits, red, turn));
   // a thread reads and writes the same channels in every pass, so sum may be x or the residual
   for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
     const float z = z_at(c);
@@ -373,24 +409,29 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   if (threadIdx.x == 0) p.row_scale[row] = s.scale;
 }
 
-// A warp per row, eight elements per lane and step.
+// A warp per piece of a row: four eights per lane, their loads under way together.
+constexpr int kDequantizeEights = 4 * 32;
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int64_t rows, int eights) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int64_t rows, int eights, int pieces) {
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = unit / pieces;
   if (row >= rows) return;
+  const int k0 = static_cast<int>(unit - row * pieces) * kDequantizeEights + (threadIdx.x & 31);
   const float s = scale[row];
   const uint2* src = reinterpret_cast<const uint2*>(q + row * q_stride);
-  const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int k = lane; k < eights; k += 32) {
-    const uint2 v = src[k];
+  uint2 v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = k0 + 32 * j < eights ? src[k0 + 32 * j] : make_uint2(0u, 0u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (k0 + 32 * j >= eights) break;
     // q + 128 in the low mantissa bits of 2^23 is 2^23 + 128 + q, exactly; the conversion instruction is slow
-    const uint32_t u[2] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u};
+    const uint32_t u[2] = {v[j].x ^ 0x80808080u, v[j].y ^ 0x80808080u};
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = (__uint_as_float(__byte_perm(u[i >> 2], 0x4b000000u, 0x7540 + (i & 3))) - 8388736.f) * s;
-    Raw8<T>::put(out, row * out_stride + 8 * k, f);
+    Raw8<T>::put(out, row * out_stride + 8 * (k0 + 32 * j), f);
   }
 }
 
