@@ -39,6 +39,23 @@ int make_map8(CUtensorMap* map, const dmf_int8_matrix& t, int rows, int k, int b
   return r == CUDA_SUCCESS ? DMF_ATTN_OK : DMF_ATTN_ERR_TENSOR_MAP;
 }
 
+// map of the result for TMA stores of 128 bytes x 32 rows
+int make_out_map(CUtensorMap* map, const dmf_int8_linear_args* a) {
+  const EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) return DMF_ATTN_ERR_DEVICE;
+  const int bytes = element_bytes(a->out_dtype);
+  const CUtensorMapDataType dt = a->out_dtype == DMF_INT8_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : a->out_dtype == DMF_INT8_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a->n), static_cast<cuuint64_t>(a->m)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a->out_stride) * bytes};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / bytes), 32}, steps[2] = {1, 1};
+  const CUresult r = encode_in_context([&] {
+    return encode(map, dt, 2, a->out, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+  return r == CUDA_SUCCESS ? DMF_ATTN_OK : DMF_ATTN_ERR_TENSOR_MAP;
+}
+
 template <typename Kernel, typename... Args>
 int launch_cluster(Kernel kernel, unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -65,7 +82,7 @@ int launch_pair_gemm(const Int8GemmParams& p, int sms, cudaStream_t stream) {
   const auto kernel = int8_gemm_pair_kernel<BN, T>;
   if (!allow_smem(kernel, Int8PairTraits<BN>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
   const int tiles = p.tiles_m * p.tiles_n, clusters = tiles < sms / 2 ? tiles : sms / 2;
-  return launch_cluster(kernel, 2u * clusters, kInt8PairThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
+  return launch_cluster(kernel, 2u * clusters, Int8PairTraits<BN>::kThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
 }
 
 template <int TB, typename T>
@@ -122,6 +139,7 @@ int run_plan(const GemmPlan& g, const dmf_int8_linear_args* a, int sms) {
   p.bias = a->bias; p.bias_dtype = a->bias_dtype;
   p.out = a->out; p.out_stride = a->out_stride; p.out_dtype = a->out_dtype;
   p.out_vec = reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && a->out_stride * element_bytes(a->out_dtype) % 16 == 0;
+  if (p.out_vec && !g.few && (st = make_out_map(&p.out_map, a)) != DMF_ATTN_OK) return st;
   p.status_word = a->status_word;
   p.m = a->m; p.n = a->n; p.k = a->k;
   const int64_t tiles_m = (static_cast<int64_t>(a->m) + (g.few ? g.tile : 256) - 1) / (g.few ? g.tile : 256);

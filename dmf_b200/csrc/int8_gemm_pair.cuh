@@ -6,10 +6,14 @@
 // M = 256, N = BN, 32 bytes of k each.  CTA r holds 128 of the tile's rows of x and half of its rows of w, so a 128-byte step of
 // k costs each SM 16 KB + BN / 2 * 128 bytes of loads for 256 x BN x 128 products of the pair.
 //
-// Warps: 0 TMA producer (both CTAs), 1 MMA issuer (leader CTA), 2..9 epilogue (both CTAs).  Two accumulators of BN columns
+// Warps: 0 TMA producer (both CTAs), 1 MMA issuer (leader CTA), 2.. epilogue (both CTAs).  Two accumulators of BN columns
 // alternate in tensor memory, so the epilogue of a tile runs under the products of the next one.  An epilogue warp takes 32 rows
-// (its quarter of the lanes) and half of the columns: scales and bias from a copy of its own in shared memory, the rounded
-// results through 4 KB of its own to whole 16-byte pieces of rows, 128 bytes of a row at a time.
+// (its quarter of the lanes) and 64 or 128 columns, 64 at a time; the rounded results go through 4 KB of its own to a TMA store.
+//
+// What bounds it: shared memory.  At full rate the loads write 64 bytes per cycle and SM and the products read as much, of the
+// 128 it has, so the epilogue has to be sparing: it reads the accumulators in the layout of matrix fragments, where a thread has
+// two columns of each eight and so reads 16 bytes of scales and bias for eight results.  (In the row layout, where every thread
+// reads those of all columns, that alone took 6 us of 59 at 16384 x 1152 x 3456.)
 //
 // Every wait is bounded (see sm100_ptx.cuh); a role whose wait gives up leaves its loop, the others follow at their next wait,
 // all meet at the end.
@@ -27,6 +31,7 @@ namespace dmf {
 
 struct Int8GemmParams {
   CUtensorMap x_map, w_map;     // boxes of 128 bytes of k; x: 128 rows (pair) / the tile's tokens, w: BN / 2 rows (pair) / 128
+  CUtensorMap out_map;          // pair, out_vec: boxes of 128 bytes x 32 rows
   const float *x_scale, *w_scale;
   const void* bias;
   void* out;
@@ -39,22 +44,6 @@ struct Int8GemmParams {
 };
 
 constexpr int kRoleInt8Producer = 600, kRoleInt8Mma = 700, kRoleInt8Epilogue = 800;
-
-// the output type's vectors: 16 bytes of results
-template <typename T>
-struct OutVec {
-  static constexpr int kElems = 8;
-  __device__ __forceinline__ static uint4 pack(const float* v) {
-    return make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]), Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
-  }
-};
-template <>
-struct OutVec<float> {
-  static constexpr int kElems = 4;
-  __device__ __forceinline__ static uint4 pack(const float* v) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  }
-};
 
 // After a wait gave up: loads that were issued land before anybody reuses or leaves the shared memory (they need microseconds;
 // the wait that gave up has taken seconds).
@@ -70,15 +59,16 @@ struct Int8PairTraits {
   static constexpr int kXBytes = 128 * 128, kWBytes = BN / 2 * 128, kStageBytes = kXBytes + kWBytes;
   static constexpr int kStages = BN == 256 ? 5 : (BN == 192 ? 6 : 7);
   static constexpr int kRingBytes = kStages * kStageBytes;
-  static constexpr int kWarpStage = 4096, kWarpVec = BN / 2 * 8;       // per epilogue warp: staged results; scales and bias
+  static constexpr int kCols = BN == 256 ? 128 : 64;                   // columns of an epilogue warp
+  static constexpr int kWarps = BN / kCols * 4, kThreads = 64 + 32 * kWarps;   // epilogue warps; all threads
+  static constexpr int kWarpStage = 4096, kWarpVec = kCols * 8;        // per epilogue warp: staged results; scales and bias
   static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = kBarAccFull + 2,
                        kNumBars = kBarAccEmpty + 2;
-  static constexpr int kSmemBytes = 1024 + kRingBytes + 8 * (kWarpStage + kWarpVec) + kNumBars * 8 + 16;
+  static constexpr int kSmemBytes = 1024 + kRingBytes + kWarps * (kWarpStage + kWarpVec) + kNumBars * 8 + 16;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
   static constexpr uint32_t kTmemCols = BN == 128 ? 256 : 512;
 };
 
-constexpr int kInt8PairThreads = 320;
 constexpr int kInt8GroupM = 8;   // tiles run over w within groups of 8 row tiles: w is read from HBM once per 2048 rows at most
 
 __device__ __forceinline__ void int8_tile(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
@@ -90,14 +80,14 @@ __device__ __forceinline__ void int8_tile(int t, int tiles_m, int tiles_n, int& 
 }
 
 template <int BN, typename T>
-__global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(const __grid_constant__ Int8GemmParams p) {
+__global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pair_kernel(const __grid_constant__ Int8GemmParams p) {
   using TR = Int8PairTraits<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t s_ring = smem_u32(smem);
   uint8_t* out_stage = smem + TR::kRingBytes;
-  uint8_t* vecs = out_stage + 8 * TR::kWarpStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(vecs + 8 * TR::kWarpVec);
+  uint8_t* vecs = out_stage + TR::kWarps * TR::kWarpStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(vecs + TR::kWarps * TR::kWarpVec);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + TR::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t bar0 = smem_u32(bars);
@@ -114,7 +104,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(con
     for (int i = 0; i < TR::kNumBars; ++i) {
       uint32_t count = 1;                          // tcgen05.commit, multicast from the leader
       if (i < TR::kBarEmpty) count = 2;            // the producers' arrivals with their bytes (used in the leader)
-      if (i >= TR::kBarAccEmpty) count = 16;       // the epilogue warps of both CTAs (used in the leader)
+      if (i >= TR::kBarAccEmpty) count = 2 * TR::kWarps;  // the epilogue warps of both CTAs (used in the leader)
       mbar_init(bar(i), count);
     }
     fence_mbar_init();
@@ -184,39 +174,43 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(con
     }
   } else {
     // =========================== epilogue (each CTA) ==========================
-    constexpr int kCols = BN / 2;                      // columns of a warp
-    constexpr int kVec = OutVec<T>::kElems;            // results per 16 bytes
-    constexpr int kPer = kCols / 32;                   // columns of a lane's scales
-    const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
+    constexpr int kCols = TR::kCols, kPer = kCols / 32;
+    constexpr int kWide = 128 / sizeof(T);             // results per 128 bytes: 64 or 32
+    const int ew = warp - 2, quarter = warp & 3, col0 = (ew >> 2) * kCols;
     float* s_w = reinterpret_cast<float*>(vecs + ew * TR::kWarpVec);
     float* s_b = s_w + kCols;
     uint8_t* stage = out_stage + ew * TR::kWarpStage;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kCols;
-    // scales and bias of a tile's columns and the scale of this lane's row: in registers a tile ahead
-    float next_w[kPer], next_b[kPer], next_x = 0.f;
+    const uint32_t s_stage = smem_u32(stage);
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
+    const int frow = lane >> 2, fcol = 2 * (lane & 3);  // this lane's first row and column of a fragment
+    // scales and bias of a tile's columns and the scales of this lane's rows: in registers a tile ahead
+    float next_w[kPer], next_b[kPer], next_x[4];
     auto fetch = [&](int t) {
       if (t >= tiles) return;
       int tm, tn;
       int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
-      const int n0 = tn * BN + half * kCols;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int n = n0 + i * 32 + lane;
+        const int n = tn * BN + col0 + i * 32 + lane;
         next_w[i] = n < p.n ? p.w_scale[n] : 0.f;
         next_b[i] = n < p.n && p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n) : 0.f;
       }
-      const int64_t m = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32 + lane;
-      next_x = m < p.m ? p.x_scale[m] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t m = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32 + frow + 8 * i;
+        next_x[i] = m < p.m ? p.x_scale[m] : 0.f;
+      }
     };
+    auto slot = [](int row, int piece) -> int { return row * 128 + ((piece ^ (row & 7)) << 4); };   // the store map's swizzle
     fetch(cluster_id);
     uint32_t tcnt = 0;
     for (int t = cluster_id; t < tiles; t += num_clusters, ++tcnt) {
       int tm, tn;
       int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
-      const int n0 = tn * BN + half * kCols;
-      const int64_t m0 = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32;
+      const int n0 = tn * BN + col0;
+      const int m0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
       const uint32_t a = tcnt & 1u;
-      const float xs = next_x;
+      const float xs[4] = {next_x[0], next_x[1], next_x[2], next_x[3]};
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         s_w[i * 32 + lane] = next_w[i];
@@ -228,75 +222,63 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1) int8_gemm_pair_kernel(con
                                                         kRoleInt8Epilogue + TR::kBarAccFull + a));
       if (!ok) break;
       tc_fence_after_sync();
-      const bool whole = p.out_vec && m0 + 32 <= p.m && n0 + kCols <= p.n;
-      // W columns from column c0 of this warp: at most 128 bytes of each row go through shared memory at a time
-      auto emit = [&](int c0, auto width) {
-        constexpr int W = decltype(width)::value;
-        constexpr int kPieces = W / kVec;              // 16-byte pieces of a row, 8 or 4
-        constexpr int kRows = 32 / kPieces;            // rows per warp-wide store
-        auto slot = [](int row, int piece) -> int {
-          return row * (kPieces * 16) + ((piece ^ (kPieces == 8 ? row & 7 : (row >> 1) & 3)) << 4);
-        };
 #pragma unroll
-        for (int h = 0; h < W / 32; ++h) {
-          const int c = c0 + h * 32;
-          uint32_t v[32];
-          tmem_ld_x32(lane_base + a * BN + c, v);
-          float4 w4[8], b4[8];                         // under the load: all before the stores, which could alias them
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            w4[i] = *reinterpret_cast<const float4*>(s_w + c + 4 * i);
-            b4[i] = *reinterpret_cast<const float4*>(s_b + c + 4 * i);
-          }
-          tmem_wait_ld();
-          if (c + 32 == kCols) {                       // the tile's last read: the accumulator may be written again
-            tc_fence_before_sync();
-            mbar_arrive_warp_cluster(lbar(TR::kBarAccEmpty + a));
-          }
-          float f[32];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            f[4 * i] = fmaf(static_cast<float>(static_cast<int>(v[4 * i])) * xs, w4[i].x, b4[i].x);
-            f[4 * i + 1] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 1])) * xs, w4[i].y, b4[i].y);
-            f[4 * i + 2] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 2])) * xs, w4[i].z, b4[i].z);
-            f[4 * i + 3] = fmaf(static_cast<float>(static_cast<int>(v[4 * i + 3])) * xs, w4[i].w, b4[i].w);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += kVec)
-            *reinterpret_cast<uint4*>(stage + slot(lane, (h * 32 + j) / kVec)) = OutVec<T>::pack(f + j);
+      for (int c0 = 0; c0 < kCols; c0 += 32) {
+        uint32_t lo[16], hi[16];                       // rows frow, + 8 and + 16, + 24
+        tmem_ld_16x256b_x4(lane_base + a * BN + c0, lo);
+        tmem_ld_16x256b_x4(lane_base + (16u << 16) + a * BN + c0, hi);
+        if (c0 % kWide == 0) {                         // the stage: its last store has read it
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
         }
-        __syncwarp();
-        const int row0 = lane / kPieces, piece = lane % kPieces;
-        T* dst = static_cast<T*>(p.out) + (m0 + row0) * p.out_stride + n0 + c0 + piece * kVec;
-        if (whole) {
-          uint4 v[kPieces];
+        tmem_wait_ld();
+        if (c0 + 32 == kCols) {                        // the accumulator may be written again
+          tc_fence_before_sync();
+          mbar_arrive_warp_cluster(lbar(TR::kBarAccEmpty + a));
+        }
 #pragma unroll
-          for (int it = 0; it < kPieces; ++it) v[it] = *reinterpret_cast<const uint4*>(stage + slot(it * kRows + row0, piece));
+        for (int j = 0; j < 4; ++j) {
+          const float2 w = *reinterpret_cast<const float2*>(s_w + c0 + 8 * j + fcol), b = *reinterpret_cast<const float2*>(s_b + c0 + 8 * j + fcol);
+          float f[4][2];                               // rows frow + 8 i
 #pragma unroll
-          for (int it = 0; it < kPieces; ++it) *reinterpret_cast<uint4*>(dst + it * kRows * p.out_stride) = v[it];
-        } else {
-          const int n = n0 + c0 + piece * kVec;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t* v = (i < 2 ? lo : hi) + 4 * j + 2 * (i & 1);
+            f[i][0] = fmaf(static_cast<float>(static_cast<int>(v[0])) * xs[i], w.x, b.x);
+            f[i][1] = fmaf(static_cast<float>(static_cast<int>(v[1])) * xs[i], w.y, b.y);
+          }
+          if constexpr (sizeof(T) == 2) {
+            stmatrix_x4(s_stage + slot(lane, (c0 % kWide) / 8 + j), Pack2<T>::pack(f[0][0], f[0][1]), Pack2<T>::pack(f[1][0], f[1][1]),
+                        Pack2<T>::pack(f[2][0], f[2][1]), Pack2<T>::pack(f[3][0], f[3][1]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float2*>(stage + slot(frow + 8 * i, 2 * j + (fcol >> 2)) + (fcol & 2) * 4) = make_float2(f[i][0], f[i][1]);
+          }
+        }
+        if ((c0 + 32) % kWide == 0) {                  // 128 bytes of every row are staged
+          const int n = n0 + c0 + 32 - kWide;
+          if (p.out_vec) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&p.out_map, s_stage, n, m0);   // clipped at the matrix's ends
+              tma_store_commit();
+            }
+          } else {
+            __syncwarp();
 #pragma unroll 1
-          for (int it = 0; it < kPieces; ++it, dst += kRows * p.out_stride) {
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + slot(it * kRows + row0, piece));
-            if (m0 + it * kRows + row0 >= p.m) continue;
-            if (p.out_vec && n + kVec <= p.n) {
-              *reinterpret_cast<uint4*>(dst) = v;
-            } else {
-              const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-              for (int i = 0; i < kVec; ++i)
-                if (n + i < p.n) dst[i] = e[i];
+            for (int i = lane; i < 32 * kWide; i += 32) {
+              const int row = i / kWide, c = i % kWide;
+              if (m0 + row < p.m && n + c < p.n)
+                static_cast<T*>(p.out)[(static_cast<int64_t>(m0) + row) * p.out_stride + n + c] =
+                    *reinterpret_cast<const T*>(stage + slot(row, c * static_cast<int>(sizeof(T)) / 16) + c * static_cast<int>(sizeof(T)) % 16);
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
-      };
-      constexpr int kWide = 8 * kVec;                  // 128 bytes of a row: 64 or 32 columns
-#pragma unroll
-      for (int c0 = 0; c0 + kWide <= kCols; c0 += kWide) emit(c0, std::integral_constant<int, kWide>{});
-      if constexpr (kCols % kWide != 0) emit(kCols / kWide * kWide, std::integral_constant<int, kCols % kWide>{});
+      }
     }
+    if (p.out_vec && lane == 0) tma_store_wait_all();
   }
 
   // ============================== teardown ==================================
