@@ -1,6 +1,7 @@
 // C ABI of inference in 8-bit integers (include/dmf_int8.h), the product: validation, choice of kernel and launches.
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstring>
 
 #include "attn_launch.h"
@@ -101,15 +102,34 @@ struct GemmPlan {
   int splits;
 };
 
+// The cut with the shortest time by a model of it in microseconds, fitted to measurements of all of them at 40 shapes of 1 to
+// 16384 rows (K 128 to 8192, N 100 to 8192).  A step of k costs what its loads take at the 102 GB/s per SM that the L2 feeds
+// all SMs with; the rest is launch, start and end of a tile, and the exchange of the sums of a split k.
+//   pair: rounds of tiles over the SM pairs, each c(bn) + steps * t(bn)
+//   few:  tiles per SM, each e(tb) + steps / splits * (128 + tb) * 128 bytes; splits only where every CTA has an SM of its own,
+//         for 0.7 + 0.0013 per CTA and column sent (distributed shared memory: 0.19 us a column with 144 CTAs sending)
 GemmPlan plan_gemm(int m, int n, int k, int sms) {
-  if (m <= 256) {
-    GemmPlan g = {true, m <= 16 ? 16 : (m <= 32 ? 32 : 64), 1};
-    const int64_t tiles = static_cast<int64_t>((m + g.tile - 1) / g.tile) * ((n + 127) / 128);
-    const int k_steps = (k + 127) / 128;
-    while (g.splits < 8 && tiles * g.splits * 2 <= sms && g.splits * 2 <= k_steps) g.splits *= 2;
-    return g;
-  }
-  return {false, 256, 1};
+  const double steps = (k + 127) / 128;
+  auto tiles = [&](int tm, int tn) { return static_cast<double>((static_cast<int64_t>(m) + tm - 1) / tm) * static_cast<double>((static_cast<int64_t>(n) + tn - 1) / tn); };
+  GemmPlan best = {false, 256, 1};
+  double least = 1e30;
+  auto consider = [&](bool few, int tile, int splits, double us) {
+    if (us < least) {
+      least = us;
+      best = {few, tile, splits};
+    }
+  };
+  struct { int bn; double c, t; } pairs[] = {{128, 0.56, 0.251}, {192, 0.93, 0.296}, {256, 0.94, 0.349}};
+  for (const auto& g : pairs) consider(false, g.bn, 1, 5.2 + std::ceil(tiles(256, g.bn) / (sms / 2)) * (g.c + steps * g.t));
+  struct { int tb; double e; } fews[] = {{16, 0.55}, {32, 0.9}, {64, 1.5}};
+  for (const auto& g : fews)
+    for (int s = 1; s <= 8 && s <= steps; s *= 2) {
+      const double count = tiles(g.tb, 128) * s;
+      if (s > 1 && count > sms) break;
+      consider(true, g.tb, s, 5.0 + std::ceil(count / sms) * (g.e + std::ceil(steps / s) * (128 + g.tb) * 128 / 102e3) +
+                                  (s > 1 ? 0.7 + 0.0013 * count * g.tb * (s - 1) / s : 0.0));
+    }
+  return best;
 }
 
 template <typename T>
@@ -118,8 +138,7 @@ int launch_gemm(const GemmPlan& g, const Int8GemmParams& p, int sms, cudaStream_
     switch (g.tile) {
       case 16: return launch_few_gemm<16, T>(p, g.splits, stream);
       case 32: return launch_few_gemm<32, T>(p, g.splits, stream);
-      case 64: return launch_few_gemm<64, T>(p, g.splits, stream);
-      default: return launch_few_gemm<128, T>(p, g.splits, stream);
+      default: return launch_few_gemm<64, T>(p, g.splits, stream);
     }
   }
   switch (g.tile) {

@@ -20,7 +20,7 @@ struct Int8FewTraits {
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kSumBytes = TB * 128 * 4;
   static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAcc = 2 * kStages, kNumBars = kBarAcc + 1;
-  static constexpr int kSmemBytes = 1024 + kRingBytes + kSumBytes + kNumBars * 8 + 16;
+  static constexpr int kSmemBytes = 1024 + kRingBytes + kSumBytes + TB * 4 + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = TB < 32 ? 32 : TB;
 };
 
@@ -32,8 +32,9 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t s_ring = smem_u32(smem);
-  int* sums = reinterpret_cast<int*>(smem + TR::kRingBytes);     // [source CTA][column of mine][channel]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TR::kRingBytes + TR::kSumBytes);
+  int* sums = reinterpret_cast<int*>(smem + TR::kRingBytes);     // [source CTA][channel][column of mine]
+  float* s_x = reinterpret_cast<float*>(smem + TR::kRingBytes + TR::kSumBytes);   // the tokens' scales
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TR::kRingBytes + TR::kSumBytes + TB * 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + TR::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t bar0 = smem_u32(bars);
@@ -108,35 +109,44 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
       ws = p.w_scale[n];
       b = p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n) : 0.f;
     }
+    if (threadIdx.x - 64 < TB) s_x[threadIdx.x - 64] = m0 + static_cast<int>(threadIdx.x) - 64 < p.m ? p.x_scale[m0 + threadIdx.x - 64] : 0.f;
+    named_bar_sync(1, 128);
     ok = __all_sync(0xffffffffu, mbar_wait(bar(TR::kBarAcc), 0, abort_flag, p.status_word, kRoleInt8Epilogue + TR::kBarAcc));
     tc_fence_after_sync();
   }
-  auto put = [&](int m, int sum) {
-    if (mine && m < p.m) {
-      const float y = fmaf(static_cast<float>(sum) * p.x_scale[m], ws, b);
-      if constexpr (std::is_same<T, float>::value) out[m * p.out_stride] = y;
-      else out[m * p.out_stride] = T(y);
+  auto put = [&](int col, int sum) {
+    const float y = fmaf(static_cast<float>(sum) * s_x[col], ws, b);
+    if (mine && m0 + col < p.m) {
+      T* dst = out + static_cast<int64_t>(m0 + col) * p.out_stride;
+      if constexpr (std::is_same<T, float>::value) *dst = y;
+      else *dst = T(y);
     }
   };
   constexpr int kChunk = TB < 32 ? TB : 32;
-  const int cols = TB / splits, shift = __ffs(cols) - 1;   // columns of a CTA: a power of two
+  const int cols = TB / splits, shift = __ffs(cols) - 1;   // columns of a CTA: a power of two, 2 at least
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   if (ok) {
 #pragma unroll
     for (int c0 = 0; c0 < TB; c0 += kChunk) {
+      if (m0 + c0 >= p.m) break;
       uint32_t v[kChunk];
       if constexpr (kChunk == 16) tmem_ld_x16(lane_base + c0, v);
       else tmem_ld_x32(lane_base + c0, v);
       tmem_wait_ld();
       if (splits == 1) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) put(m0 + c0 + j, static_cast<int>(v[j]));
+        for (int j = 0; j < kChunk; ++j) put(c0 + j, static_cast<int>(v[j]));
       } else {
+        // to the column's owner, columns of one channel side by side; tokens that are none travel too, nobody reads them
+        auto at = [&](int c) -> uint32_t {
+          return map_to_cta(smem_u32(sums + (rank * 128 + channel) * cols + (c & (cols - 1))), c >> shift);
+        };
+        if (cols >= 4) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const int owner = (c0 + j) >> shift, col = (c0 + j) & (cols - 1);
-          if (m0 + c0 + j < p.m)
-            st_shared_cluster_u32(map_to_cta(smem_u32(sums + (rank * cols + col) * 128 + channel), owner), v[j]);
+          for (int j = 0; j < kChunk; j += 4) st_shared_cluster_v4(at(c0 + j), v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kChunk; j += 2) st_shared_cluster_v2(at(c0 + j), v[j], v[j + 1]);
         }
       }
     }
@@ -145,10 +155,10 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
     __syncwarp();
     cluster_sync_all();                          // everybody's sums have arrived
     if (ok)
-      for (int col = 0; col < cols; ++col) {
+      for (int c = 0; c < cols && m0 + rank * cols + c < p.m; ++c) {
         int s = 0;
-        for (int r = 0; r < splits; ++r) s += sums[(r * cols + col) * 128 + channel];
-        put(m0 + rank * cols + col, s);
+        for (int r = 0; r < splits; ++r) s += sums[(r * 128 + channel) * cols + c];
+        put(rank * cols + c, s);
       }
   }
   __syncwarp();
