@@ -156,10 +156,21 @@ __device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, fl
   }
 }
 
+// row_act of eight elements, two to an instruction where there is one for two
 template <int kAct>
 __device__ __forceinline__ void row_act8(float (&f)[8]) {
+  constexpr float kLog2e = 1.4426950408889634f, c1 = -2.f * 0.7978845608028654f * kLog2e;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = row_act<kAct>(f[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t x = pack_f2(f[i], f[i + 1]);
+    uint64_t v;
+    if constexpr (kAct == 1) v = mul2(x, fma2(pack_f2(c1 * 0.044715f, c1 * 0.044715f), mul2(x, x), pack_f2(c1, c1)));
+    else v = mul2(pack_f2(-kLog2e, -kLog2e), x);
+    float v0, v1, d0, d1;
+    unpack_f2(v, v0, v1);
+    unpack_f2(add2(pack_f2(1.f, 1.f), pack_f2(fast_exp2(v0), fast_exp2(v1))), d0, d1);
+    unpack_f2(mul2(x, pack_f2(row_rcp(d0), row_rcp(d1))), f[i], f[i + 1]);
+  }
 }
 
 // A row in registers, thread `t` of `threads` holding eights t, t + threads, ...
@@ -268,7 +279,12 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoad
       if (!zeros) {
         uint32_t u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = row_quantize(z[k][i], rs.inverse);
+        for (int i = 0; i < 8; i += 2) {   // row_quantize of two
+          float a, b;
+          unpack_f2(add2(mul2(pack_f2(z[k][i], z[k][i + 1]), pack_f2(rs.inverse, rs.inverse)), pack_f2(12582912.f, 12582912.f)), a, b);
+          u[i] = __float_as_uint(a);
+          u[i + 1] = __float_as_uint(b);
+        }
         out = make_uint2(row_pack4(u[0], u[1], u[2], u[3]), row_pack4(u[4], u[5], u[6], u[7]));
       }
       *reinterpret_cast<uint2*>(q + 8 * (t + k * threads)) = out;
