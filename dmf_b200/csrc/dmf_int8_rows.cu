@@ -111,7 +111,7 @@ constexpr int kNoKernel = -1;   // of launch_types: a pair of types without a ke
 
 template <int kOp, typename TX>
 int launch_types(const Int8RowParams& p, int sms, cudaStream_t stream) {
-  if constexpr (kOp != kRowQuantize) {
+  if constexpr (kIsNorm<kOp>) {
     if (p.add != nullptr) {
       constexpr bool kF32 = std::is_same<TX, float>::value;
       if (p.add_dtype == DMF_INT8_F32) return launch_vectors<kOp, TX, float>(p, sms, stream);
@@ -163,9 +163,14 @@ int run_quantize(const dmf_int8_quantize_args* a) {
   }
   Int8RowParams p = {};
   p.x = a->x.ptr; p.x_sb = a->x.stride_b; p.x_sl = a->x.stride_l; p.x_dtype = a->dtype;
-  p.rows = rows; p.batch = a->batch; p.seqlen = a->seqlen; p.channels = a->channels; p.act = a->act;
+  p.rows = rows; p.batch = a->batch; p.seqlen = a->seqlen; p.channels = a->channels;
   set_out(&p, a->out);
-  return launch_rows<kRowQuantize>(p, static_cast<cudaStream_t>(a->stream));
+  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+  switch (a->act) {
+    case DMF_INT8_ACT_GELU: return launch_rows<kRowGelu>(p, stream);
+    case DMF_INT8_ACT_SILU: return launch_rows<kRowSilu>(p, stream);
+    default: return launch_rows<kRowQuantize>(p, stream);
+  }
 }
 
 int run_rmsnorm(const dmf_int8_rmsnorm_args* a) {

@@ -22,7 +22,11 @@
 
 namespace dmf {
 
-enum Int8RowOp { kRowQuantize = 0, kRowRms = 1, kRowLn = 2 };
+enum Int8RowOp { kRowQuantize, kRowGelu, kRowSilu, kRowRms, kRowLn };
+template <int kOp>
+constexpr bool kIsNorm = kOp == kRowRms || kOp == kRowLn;
+template <int kOp>
+constexpr int kActOf = kOp == kRowGelu ? 1 : (kOp == kRowSilu ? 2 : 0);
 
 struct Int8RowParams {
   const void *x, *add;                  // add: residual (RMS) or h (LayerNorm); nullptr: none
@@ -35,7 +39,6 @@ struct Int8RowParams {
   int64_t rows;
   int seqlen, channels, batch;
   int x_dtype, add_dtype, sum_dtype, mod_dtype;   // mod: weight / gate, shift, scale
-  int act;
   float eps;
 };
 
@@ -156,7 +159,11 @@ __device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, fl
   }
 }
 
-// row_act of eight elements, two to an instruction where there is one for two
+// row_act of eight elements, two to an instruction where there is one for two and with one reciprocal for two: 1 / d0 and 1 / d1
+// are d1 r and d0 r with r = 1 / (d0 d1), which halves the reciprocals, whose unit bounds these activations (16 results a clock
+// and SM, for them and the exponentials).  v is held at 63 so that the product stays finite; where that matters the true result is
+// below |x| 2^-63, so the caller looks at the row's maximum and takes row_act for rows below kRowActExact.
+constexpr float kRowActExact = 9.094947017729282e-13f;   // 2^-40
 template <int kAct>
 __device__ __forceinline__ void row_act8(float (&f)[8]) {
   constexpr float kLog2e = 1.4426950408889634f, c1 = -2.f * 0.7978845608028654f * kLog2e;
@@ -168,8 +175,9 @@ __device__ __forceinline__ void row_act8(float (&f)[8]) {
     else v = mul2(pack_f2(-kLog2e, -kLog2e), x);
     float v0, v1, d0, d1;
     unpack_f2(v, v0, v1);
-    unpack_f2(add2(pack_f2(1.f, 1.f), pack_f2(fast_exp2(v0), fast_exp2(v1))), d0, d1);
-    unpack_f2(mul2(x, pack_f2(row_rcp(d0), row_rcp(d1))), f[i], f[i + 1]);
+    unpack_f2(add2(pack_f2(1.f, 1.f), pack_f2(fast_exp2(fminf(v0, 63.f)), fast_exp2(fminf(v1, 63.f)))), d0, d1);
+    const float r = row_rcp(d0 * d1);
+    unpack_f2(mul2(x, mul2(pack_f2(d1, d0), pack_f2(r, r))), f[i], f[i + 1]);
   }
 }
 
@@ -195,7 +203,7 @@ struct RowLoads {
 //   load_next: called once the loads are in z;  sum_up, max_up: over the row's threads
 //   vec(which, c, f): eight channels of 0 gate, 1 weight or 1 + scale, 2 shift
 template <int kOp, typename TX, typename TA, int NV, typename Next, typename SumUp, typename MaxUp, typename Vec>
-__device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoads<kOp, TX, TA, NV>& loads, int64_t row, int64_t sum0, int t,
+__device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoads<kOp, TX, TA, NV>& loads, int64_t row, int64_t x0, int64_t sum0, int t,
                                                  int threads, Next&& load_next, SumUp&& sum_up, MaxUp&& max_up, Vec&& vec) {
   using Loads = RowLoads<kOp, TX, TA, NV>;
   constexpr bool kAdd = Loads::kAdd;
@@ -227,13 +235,11 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoad
     }
   }
   load_next();
-  if constexpr (kOp == kRowQuantize) {
+  if constexpr (kActOf<kOp> != 0) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (p.act == 1) row_act8<1>(z[k]);
-      else if (p.act == 2) row_act8<2>(z[k]);
-    }
-  } else {
+    for (int k = 0; k < NV; ++k) row_act8<kActOf<kOp>>(z[k]);
+  }
+  if constexpr (kIsNorm<kOp>) {
     const float inv_c = 1.f / static_cast<float>(p.channels);
     if constexpr (kOp == kRowLn) {
 #pragma unroll
@@ -269,7 +275,26 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoad
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int i = 0; i < 8; i += 2) top = row_max3(top, z[k][i], z[k][i + 1]);
-  const RowScale rs = row_scale_of(max_up(__float_as_uint(top)));
+  uint32_t bits = max_up(__float_as_uint(top));
+  if constexpr (kActOf<kOp> != 0) {
+    if (bits < __float_as_uint(kRowActExact)) {   // (the whole row alike)
+      top = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (t + k * threads < eights) {
+          Raw8<TX> x;
+          x.load(p.x, x0 + 8 * (t + k * threads));
+          x.get(z[k]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            z[k][i] = row_act<kActOf<kOp>>(z[k][i]);
+            top = row_max3(top, z[k][i], z[k][i]);
+          }
+        }
+      bits = max_up(__float_as_uint(top));
+    }
+  }
+  const RowScale rs = row_scale_of(bits);
   int8_t* q = p.q + row * p.q_stride;
   const bool zeros = rs.inverse == 0.f;
 #pragma unroll
@@ -297,7 +322,7 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoad
 // block, as fp32.  (RMS norm and quantisation see all rows as one sample.)
 constexpr int kGroupThreads = 512;      // most threads of a block that works on one row
 template <int kOp, typename TA>
-constexpr int kRowVectors = kOp == kRowQuantize ? 0 : (kOp == kRowRms ? 1 : (std::is_void<TA>::value ? 2 : 3));
+constexpr int kRowVectors = !kIsNorm<kOp> ? 0 : (kOp == kRowRms ? 1 : (std::is_void<TA>::value ? 2 : 3));
 
 template <int kOp, typename TX, typename TA, int NV, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_group_kernel(const Int8RowParams p, int rows_per_block) {
@@ -343,7 +368,7 @@ __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_
   for (; l < l1; l += kStep) {
     const int64_t b = kOp == kRowLn ? b0 : l / p.seqlen, i = kOp == kRowLn ? l : l % p.seqlen;
     row_in_registers<kOp, TX, TA, NV>(
-        p, loads, b0 * per_sample + l, b * p.sum_sb + i * p.sum_sl, t, threads,
+        p, loads, b0 * per_sample + l, b * p.x_sb + i * p.x_sl, b * p.sum_sb + i * p.sum_sl, t, threads,
         [&] {
           if (l + kStep < l1) start(l + kStep);
         },
@@ -362,7 +387,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
   RowLoads<kOp, TX, TA, NV> loads;
   loads.start(p, b * p.x_sb + l * p.x_sl, b * p.add_sb + l * p.add_sl, threadIdx.x, blockDim.x);
   row_in_registers<kOp, TX, TA, NV>(
-      p, loads, row, b * p.sum_sb + l * p.sum_sl, threadIdx.x, blockDim.x, [] {}, [&](float v) { return row_block_sum(v, red, turn); },
+      p, loads, row, b * p.x_sb + l * p.x_sl, b * p.sum_sb + l * p.sum_sl, threadIdx.x, blockDim.x, [] {}, [&](float v) { return row_block_sum(v, red, turn); },
       [&](uint32_t v) { return row_block_max(v, red, turn); },
       [&](int which, int c, float (&f)[8]) {
         if (which == 0) row_vec8(p.gate, p.mod_dtype, b * p.gate_sb + c, f);
@@ -386,7 +411,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   const float inv_c = 1.f / static_cast<float>(p.channels);
   auto z_at = [&](int c) -> float {
     const float x = row_load(p.x, p.x_dtype, x0 + c);
-    if constexpr (kOp == kRowQuantize) return p.act == 1 ? row_act<1>(x) : (p.act == 2 ? row_act<2>(x) : x);
+    if constexpr (!kIsNorm<kOp>) return row_act<kActOf<kOp>>(x);
     if (p.add == nullptr) return x;
     const float a = row_load(p.add, p.add_dtype, add0 + c);
     if constexpr (kOp == kRowRms) return a + x;
@@ -398,7 +423,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
     for (int c = threadIdx.x; c < p.channels; c += kRowThreads) s += z_at(c);
     mean = row_block_sum(s, red, turn) * inv_c;
   }
-  if constexpr (kOp != kRowQuantize) {
+  if constexpr (kIsNorm<kOp>) {
     float s = 0.f;
     for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
       const float z = z_at(c) - mean;
@@ -407,7 +432,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
     r = rsqrtf(row_block_sum(s, red, turn) * inv_c + p.eps);
   }
   auto y_of = [&](float z, int c) -> float {
-    if constexpr (kOp == kRowQuantize) return z;
+    if constexpr (!kIsNorm<kOp>) return z;
     if constexpr (kOp == kRowRms) return z * r * row_load(p.weight, p.mod_dtype, c);
     return fmaf((z - mean) * r, 1.f + row_load(p.scale, p.mod_dtype, b * p.scale_sb + c),
                 row_load(p.shift, p.mod_dtype, b * p.shift_sb + c));
@@ -419,7 +444,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   // a thread reads and writes the same channels in every pass, so sum may be x or the residual
   for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
     const float z = z_at(c);
-    if (kOp != kRowQuantize && p.sum != nullptr) row_store(p.sum, p.sum_dtype, sum0 + c, z);
+    if (kIsNorm<kOp> && p.sum != nullptr) row_store(p.sum, p.sum_dtype, sum0 + c, z);
     p.q[row * p.q_stride + c] = static_cast<int8_t>(s.inverse == 0.f ? 0u : row_quantize(y_of(z, c), s.inverse) & 0xffu);
   }
   if (threadIdx.x == 0) p.row_scale[row] = s.scale;

@@ -9,8 +9,8 @@ TINY = 2.0 ** -120
 
 def act(x, name):
     x = x.double()
-    if name == "gelu":
-        return 0.5 * x * (1 + torch.tanh((2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3)))
+    if name == "gelu":      # 0.5 x (1 + tanh u) as x sigmoid(2 u): 1 + tanh u loses all its digits below u = -18
+        return x * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3))
     return x * torch.sigmoid(x) if name == "silu" else x
 
 

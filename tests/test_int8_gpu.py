@@ -103,6 +103,30 @@ def test_rows_of_zeros_tiny_values_and_large_ones():
     assert not ln.values.any()
 
 
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("C", [96, 1152, 4608])
+def test_activations_at_their_ends(act, C):
+    """rows whose results are tiny, nothing or as large as the type's largest"""
+    x = _randn(12, C, std=0.3)
+    x[0] -= 12.0                      # results of 1e-30 and less
+    x[1] = -8.0 - x[1].abs()
+    x[2] = -100.0
+    x[3] = 3e38
+    x[3, 1::2] = -3e38
+    x[4] = -40.0
+    x[4, 7] = 1e-14                   # the row's maximum is far below the activations' own limits
+    x[5] = -9.0
+    x[5, 0] = 5.0
+    y = orc.act(x, act)
+    for rows in (quantize_int8(x, act), Int8Rows(*(t.view(12, *t.shape[2:]) for t in quantize_int8(x.view(4, 3, C), act)))):
+        real, scale = orc.real_rows(y)
+        # exp(v) within (2 + 1.2 |v|) steps, and |v| may reach 88 where a row has nothing larger: 150 u
+        some = scale > 0
+        assert torch.equal(rows.scale > 0, some)
+        assert float((rows.values.double() - real)[some].abs().max()) <= 0.5 + 127 * 150 * U
+        assert bool(((rows.scale.double() - scale).abs() <= scale * 150 * U).all())
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("C", [40, 1152, 1153])
 def test_a_value_that_is_not_finite_spoils_its_row_and_no_other(bad, C):
