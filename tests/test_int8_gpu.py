@@ -393,3 +393,73 @@ def test_the_registered_ops_give_the_native_paths_bits():
     for native, general in pairs:
         for a, b in zip(native, general):
             assert a.stride() == b.stride() and torch.equal(a, b)
+
+
+# ---- the model in 8 bits ----------------------------------------------------------------------------------------------
+
+def _model(name="DMFT-S/2", **kw):
+    from dmf_b200.harness.model import build_dmft
+    torch.manual_seed(0)
+    kw = dict(dict(input_size=32, dmf_depth=8, num_classes=1000, attn_func="fa3", use_logvar=False, qk_norm=False), **kw)
+    model = build_dmft(name, **kw)
+    model.initialize_weights(zero_init=False)      # zero gates would hide the blocks
+    return model.to(DEV).requires_grad_(False).eval()
+
+
+# A layer's two operands are off by (a / rms) / 127 / sqrt(12) each, a the row's largest value: a / rms is about 4 behind a norm, 6
+# behind GELU, 1.7 for a weight, so 1.0 % of a product behind a norm or the attention and 1.5 % behind GELU.  qkv, attention and
+# proj in one branch, fc1 and fc2 in the other, and the modulation of both: at most 2.5 % of a branch in quadrature; the sum over
+# the blocks grows no faster than the branches themselves.  Twice that, and 1 % for the 16-bit model it is compared with.
+MODEL_TOL = 0.06
+
+
+@pytest.mark.parametrize("dtype,kw", [(BF16, {}), (BF16, {"qk_norm": True}), (F32, {})])
+def test_model_in_8_bits_is_near_the_model(dtype, kw):
+    from dmf_b200.harness.int8_model import int8_model
+    model = _model(**kw).to(dtype)
+    state = {k: v.clone() for k, v in model.state_dict().items()}
+    quantised = int8_model(model)
+    assert all(torch.equal(v, state[k]) for k, v in model.state_dict().items()) and len(model.blocks) == 12
+    x, y = _randn(4, 4, 32, 32, dtype=dtype), torch.randint(0, 1000, (4,), device=DEV)
+    t, r = torch.rand(4, device=DEV, dtype=dtype) * 0.5 + 0.5, torch.rand(4, device=DEV, dtype=dtype) * 0.5
+    with torch.no_grad(), torch.autocast("cuda", BF16, enabled=dtype == F32):
+        got, ref = quantised(x, t, r, y), model(x, t, r, y)
+    assert got.dtype == ref.dtype and got.shape == ref.shape
+    assert float((got.double() - ref.double()).norm() / ref.double().norm()) < MODEL_TOL
+
+
+def test_sampler_in_8_bits_eager_and_graphed():
+    from dmf_b200.harness.int8_model import int8_model
+    from dmf_b200.harness.sampler import GraphedSampler, euler_sampler
+    model = _model().bfloat16()
+    quantised = int8_model(model)
+    z, y = _randn(2, 4, 32, 32, dtype=BF16), torch.randint(0, 1000, (2,), device=DEV)
+    out = euler_sampler(quantised, z, y, num_steps=2, cfg_scale=1.5)
+    ref = euler_sampler(model, z, y, num_steps=2, cfg_scale=1.5)
+    # two steps, of which guidance weighs the branches with 1.5 and -0.5
+    assert float((out - ref).norm() / ref.norm()) < 2 * 1.6 * MODEL_TOL
+    graphed = GraphedSampler(quantised, 2, latent_shape=(4, 32, 32), num_steps=2, cfg_scale=1.5)
+    assert torch.equal(graphed(z, y), out)
+    z2 = _randn(2, 4, 32, 32, dtype=BF16, seed=5)
+    assert torch.equal(graphed(z2, y), euler_sampler(quantised, z2, y, num_steps=2, cfg_scale=1.5))
+
+
+def test_model_in_8_bits_moves_and_casts_without_touching_its_scales():
+    from dmf_b200.harness.int8_model import int8_model
+    quantised = int8_model(_model().bfloat16())
+    layer = quantised.blocks[0].qkv
+    values, scale = layer.values.clone(), layer.scale.clone()
+    quantised.bfloat16()
+    assert layer.scale.dtype == F32 and torch.equal(layer.scale, scale) and torch.equal(layer.values, values)
+    quantised.cpu().to(DEV)
+    assert torch.equal(layer.scale, scale) and torch.equal(layer.values, values)
+
+
+def test_model_refusals():
+    from dmf_b200.harness.int8_model import int8_model
+    with pytest.raises(ValueError, match="fa2"):
+        int8_model(_model(attn_func="base"))
+    with pytest.raises(ValueError, match="GPU"):
+        int8_model(_model().cpu())
+    with pytest.raises(ValueError, match="fp32 or bf16"):
+        int8_model(_model().half())
