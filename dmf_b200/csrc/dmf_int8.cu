@@ -10,6 +10,7 @@
 #include "int8_gemm_few.cuh"
 #include "int8_gemm_pair.cuh"
 #include "int8_launch.h"
+#include "int8_launch.h"
 #include "int8_linear.cuh"
 #include "tensor_map.h"
 
@@ -57,33 +58,13 @@ int make_out_map(CUtensorMap* map, const dmf_int8_linear_args* a) {
   return r == CUDA_SUCCESS ? DMF_ATTN_OK : DMF_ATTN_ERR_TENSOR_MAP;
 }
 
-template <typename Kernel, typename... Args>
-int launch_cluster(Kernel kernel, unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return DMF_ATTN_ERR_LAUNCH;
-  }
-  return DMF_ATTN_OK;
-}
-
 template <int BN, typename T>
 int launch_pair_gemm(const Int8GemmParams& p, int sms, cudaStream_t stream) {
   static bool allowed[64];
   const auto kernel = int8_gemm_pair_kernel<BN, T>;
   if (!allow_smem(kernel, Int8PairTraits<BN>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
   const int tiles = p.tiles_m * p.tiles_n, clusters = tiles < sms / 2 ? tiles : sms / 2;
-  return launch_cluster(kernel, 2u * clusters, Int8PairTraits<BN>::kThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
+  return launch_dependent(kernel, dim3(2u * clusters), Int8PairTraits<BN>::kThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
 }
 
 template <int TB, typename T>
@@ -91,7 +72,7 @@ int launch_few_gemm(const Int8GemmParams& p, int splits, cudaStream_t stream) {
   static bool allowed[64];
   const auto kernel = int8_gemm_few_kernel<TB, T>;
   if (!allow_smem(kernel, Int8FewTraits<TB>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
-  return launch_cluster(kernel, static_cast<unsigned>(p.tiles_m * p.tiles_n * splits), kInt8FewThreads, Int8FewTraits<TB>::kSmemBytes,
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * splits)), kInt8FewThreads, Int8FewTraits<TB>::kSmemBytes,
                         splits, stream, p, splits);
 }
 
@@ -193,9 +174,10 @@ int run_linear_any(const dmf_int8_linear_args* a) {
     p.out_stride = a->out_stride; p.out_dtype = a->out_dtype;
     p.m = static_cast<int>(a->m - m0); p.n = a->n; p.k = a->k;
     const dim3 grid(static_cast<unsigned>(tiles_n), static_cast<unsigned>(tiles_m - t0 < kSlice ? tiles_m - t0 : kSlice));
-    int8_linear_any_kernel<<<grid, 256, 0, stream>>>(p);
+    const int st = launch_dependent(int8_linear_any_kernel, grid, 256, 0, 1, stream, p);
+    if (st != DMF_ATTN_OK) return st;
   }
-  return launched();
+  return DMF_ATTN_OK;
 }
 
 int run_linear(const dmf_int8_linear_args* a) {

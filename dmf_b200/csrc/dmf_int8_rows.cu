@@ -88,8 +88,7 @@ int launch_group(const Int8RowParams& p, int threads, int sms, cudaStream_t stre
   const int64_t units = (per_sample + unit - 1) / unit;
   const int rpb = static_cast<int>((units + splits - 1) / splits * unit);
   const dim3 grid(static_cast<unsigned>((per_sample + rpb - 1) / rpb), static_cast<unsigned>(samples));
-  kernel<<<grid, threads, smem, stream>>>(p, rpb);
-  return launched();
+  return launch_dependent(kernel, grid, threads, smem, 1, stream, p, rpb);
 }
 
 template <int kOp, typename TX, typename TA>
@@ -97,14 +96,12 @@ int launch_vectors(const Int8RowParams& p, int sms, cudaStream_t stream) {
   const int eights = p.channels / 8, wide = ((eights + 3) / 4 + 31) / 32 * 32;   // threads, four eights each
   const unsigned rows = static_cast<unsigned>(p.rows);
   if (!many_rows(p, kOp, sms)) {
-    int8_row_block_kernel<kOp, TX, TA, 1><<<rows, (eights + 31) / 32 * 32, 0, stream>>>(p);
-    return launched();
+    return launch_dependent(int8_row_block_kernel<kOp, TX, TA, 1>, dim3(rows), (eights + 31) / 32 * 32, 0, 1, stream, p);
   }
   if (eights <= 64) return launch_group<kOp, TX, TA, 2, true>(p, kRowThreads, sms, stream);
   if (eights <= kWarpRowEights) return launch_group<kOp, TX, TA, 5, true>(p, kRowThreads, sms, stream);
   if constexpr (kOp == kRowLn) return launch_group<kOp, TX, TA, 4, false>(p, wide, sms, stream);
-  int8_row_block_kernel<kOp, TX, TA, 4><<<rows, wide, 0, stream>>>(p);
-  return launched();
+  return launch_dependent(int8_row_block_kernel<kOp, TX, TA, 4>, dim3(rows), wide, 0, 1, stream, p);
 }
 
 constexpr int kNoKernel = -1;   // of launch_types: a pair of types without a kernel of its own
@@ -140,8 +137,7 @@ int launch_rows(const Int8RowParams& p, cudaStream_t stream) {
     }
     if (st != kNoKernel) return st;
   }
-  int8_row_any_kernel<kOp><<<static_cast<unsigned>(p.rows), kRowThreads, 0, stream>>>(p);
-  return launched();
+  return launch_dependent(int8_row_any_kernel<kOp>, dim3(static_cast<unsigned>(p.rows)), kRowThreads, 0, 1, stream, p);
 }
 
 void set_out(Int8RowParams* p, const dmf_int8_matrix& out) {
@@ -246,24 +242,22 @@ int run_dequantize(const dmf_int8_dequantize_args* a) {
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   const bool vectors = a->channels % 8 == 0 && reinterpret_cast<uintptr_t>(a->x.values) % 8 == 0 && (a->rows == 1 || a->x.stride % 8 == 0) &&
                        whole_vectors(a->out, a->out_dtype, 0, 1, a->out_stride, a->rows == 1 ? 1 : 2);
-  if (!vectors) {
-    int8_dequantize_any_kernel<<<static_cast<unsigned>(a->rows), kRowThreads, 0, stream>>>(
-        a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->out_dtype, a->channels);
-    return launched();
-  }
+  if (!vectors)
+    return launch_dependent(int8_dequantize_any_kernel, dim3(static_cast<unsigned>(a->rows)), kRowThreads, 0, 1, stream,
+                            static_cast<const int8_t*>(a->x.values), a->x.stride, static_cast<const float*>(a->x.scale), a->out, a->out_stride,
+                            a->out_dtype, a->channels);
   const int eights = a->channels / 8, pieces = (eights + kDequantizeEights - 1) / kDequantizeEights;
   const int64_t blocks = (a->rows * pieces + kRowThreads / 32 - 1) / (kRowThreads / 32);
   if (blocks > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;
   auto launch = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(blocks), kRowThreads, 0, stream>>>(a->x.values, a->x.stride, a->x.scale, a->out, a->out_stride, a->rows,
-                                                                      eights, pieces);
+    return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, 1, stream, static_cast<const int8_t*>(a->x.values),
+                            a->x.stride, static_cast<const float*>(a->x.scale), a->out, a->out_stride, a->rows, eights, pieces);
   };
   switch (a->out_dtype) {
-    case DMF_INT8_BF16: launch(int8_dequantize_kernel<__nv_bfloat16>); break;
-    case DMF_INT8_FP16: launch(int8_dequantize_kernel<__half>); break;
-    default: launch(int8_dequantize_kernel<float>);
+    case DMF_INT8_BF16: return launch(int8_dequantize_kernel<__nv_bfloat16>);
+    case DMF_INT8_FP16: return launch(int8_dequantize_kernel<__half>);
+    default: return launch(int8_dequantize_kernel<float>);
   }
-  return launched();
 }
 
 }  // namespace

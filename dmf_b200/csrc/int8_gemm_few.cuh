@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
   if (splits > 1) cluster_sync_all();  // the others' shared memory is theirs from here on
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {

@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
   cluster_sync_all();  // both CTAs' barriers are initialised before anybody arrives remotely
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   if (warp == 0) {
     // =========================== TMA producer (each CTA) ====================

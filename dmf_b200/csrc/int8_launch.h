@@ -48,6 +48,27 @@ inline int check_matrix(const dmf_int8_matrix& t, int columns, bool written) {
   return check_pointer(t.scale, 4);
 }
 
-inline int launched() { return cudaGetLastError() == cudaSuccess ? DMF_ATTN_OK : DMF_ATTN_ERR_LAUNCH; }
+// Launches a kernel that begins with grid_dependency_wait, so that its blocks may be set up while the grid before it ends.
+template <typename Kernel, typename... Args>
+inline int launch_dependent(Kernel kernel, dim3 grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return DMF_ATTN_ERR_LAUNCH;
+  }
+  return DMF_ATTN_OK;
+}
 
 }  // namespace dmf

@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include "int8_types.cuh"
+#include "sm100_ptx.cuh"
 
 namespace dmf {
 
@@ -26,6 +27,8 @@ constexpr int kAnyTile = 64, kAnyWords = 16;  // 64 bytes of k
 
 __global__ void __launch_bounds__(256) int8_linear_any_kernel(const Int8LinearParams p) {
   __shared__ int sx[kAnyWords][kAnyTile + 1], sw[kAnyWords][kAnyTile + 1];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kAnyTile, n0 = static_cast<int64_t>(blockIdx.x) * kAnyTile;
   int acc[4][4] = {};

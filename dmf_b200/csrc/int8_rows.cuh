@@ -328,6 +328,8 @@ template <int kOp, typename TX, typename TA, int NV, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_group_kernel(const Int8RowParams p, int rows_per_block) {
   extern __shared__ __align__(16) float s_vec[];   // kRowVectors x channels: [weight or 1 + scale | shift | gate]
   __shared__ float red[2][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, threads = kWarp ? 32 : blockDim.x;
   const int64_t b0 = blockIdx.y;
   if constexpr (kRowVectors<kOp, TA> > 0) {
@@ -381,6 +383,8 @@ __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_
 template <int kOp, typename TX, typename TA, int NV>
 __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block_kernel(const Int8RowParams p) {
   __shared__ float red[2][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   int turn = 0;
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.seqlen, l = row % p.seqlen;
@@ -404,6 +408,8 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
 template <int kOp>
 __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8RowParams p) {
   __shared__ float red[2][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   int turn = 0;
   const int64_t row = blockIdx.x;
   const int64_t b = row / p.seqlen, l = row % p.seqlen;
@@ -455,6 +461,8 @@ constexpr int kDequantizeEights = 4 * 32;
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int64_t rows, int eights, int pieces) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
   const int64_t row = unit / pieces;
   if (row >= rows) return;
@@ -478,6 +486,8 @@ int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, vo
 
 __global__ void __launch_bounds__(kRowThreads)
 int8_dequantize_any_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int dtype, int channels) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int64_t row = blockIdx.x;
   const float s = scale[row];
   for (int c = threadIdx.x; c < channels; c += kRowThreads)

@@ -530,6 +530,15 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const void* 
 }
 
 // ----------------------------------------------------------------------------
+// Programmatic dependent launch: a grid launched with the attribute may start while the grid before it in the stream still runs.
+// Nothing global is read or written ahead of grid_dependency_wait, which returns when that grid is complete and its writes are
+// visible; grid_launch_dependents lets the next grid start once every block has called it or ended.
+// ----------------------------------------------------------------------------
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ----------------------------------------------------------------------------
 // small math helpers
 // ----------------------------------------------------------------------------
 
