@@ -21,6 +21,7 @@
 #include <ATen/FuncTorchTLS.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/functorch/DynamicLayer.h>
 #include <ATen/functorch/TensorWrapper.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -1003,6 +1004,11 @@ bool int8_takes(const Tensor& t, const Tensor& x) {
 }
 bool int8_takes(const std::optional<Tensor>& t, const Tensor& x) { return !t.has_value() || int8_takes(*t, x); }
 
+// An uninitialised result on x's device, from the allocator without the dispatcher (which costs as much again).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& x) {
+  return Tensor(at::detail::empty_cuda(sizes, type, x.device(), std::nullopt));
+}
+
 bool fits_int(int64_t n) { return n <= 0x7fffffff; }
 
 // (..., C) as (B, L, C)
@@ -1049,8 +1055,8 @@ Rows8 empty_rows8(const Tensor& x) {
     strides[i] = step;
     step *= x.size(i);
   }
-  r.values = at::empty_strided(x.sizes(), strides, x.options().dtype(at::kChar));
-  r.scale = at::empty(x.sizes().slice(0, d - 1), x.options().dtype(at::kFloat));
+  r.values = Tensor(at::detail::empty_strided_cuda(x.sizes(), strides, at::kChar, x.device()));
+  r.scale = fresh(x.sizes().slice(0, d - 1), at::kFloat, x);
   r.m = {static_cast<int8_t*>(r.values.data_ptr()), pitch, r.scale.data_ptr<float>()};
   return r;
 }
@@ -1105,7 +1111,7 @@ std::optional<Triple8> rms_norm_int8(const Tensor& x, const Tensor& weight_, dou
   a.x = v.rows;
   a.weight = weight.data_ptr();
   if (residual.has_value()) {
-    total = at::empty(residual->sizes(), residual->options());
+    total = fresh(residual->sizes(), residual->scalar_type(), x);
     res = rows_view(*residual);
     sum = rows_view(*total);
     a.stream_dtype = int8_dtype(residual->scalar_type());
@@ -1153,7 +1159,7 @@ std::optional<Triple8> ln_modulate_int8(const Tensor& x, const Tensor& shift, co
   a.shift = int8_mod(shift, md, &held_shift);
   a.scale = int8_mod(scale, md, &held_scale);
   if (h.has_value()) {
-    total = at::empty(x.sizes(), x.options());
+    total = fresh(x.sizes(), x.scalar_type(), x);
     hv = rows_view(*h);
     sum = rows_view(*total);
     a.dtype = int8_dtype(h->scalar_type());
@@ -1209,7 +1215,7 @@ std::optional<Tensor> int8_linear(const Tensor& xq, const Tensor& x_scale, const
   Tensor bias;
   c10::SmallVector<int64_t, 8> shape(xq.sizes().begin(), xq.sizes().end());
   shape.back() = w.rows;
-  const Tensor out = at::empty(shape, xq.options().dtype(out_dtype));
+  const Tensor out = fresh(shape, out_dtype, xq);
   dmf_int8_linear_args a = {};
   a.m = x.rows; a.n = w.rows; a.k = x.k;
   a.out_dtype = int8_dtype(out_dtype);
@@ -1233,7 +1239,7 @@ std::optional<Tensor> dequantize_int8(const Tensor& q, const Tensor& scale, at::
   at::AutoDispatchBelowADInplaceOrView below_autograd;
   const c10::cuda::CUDAGuard device_guard(q.device());
   const MatrixView v = matrix_view(q, scale);
-  const Tensor out = at::empty(q.sizes(), q.options().dtype(dtype));
+  const Tensor out = fresh(q.sizes(), dtype, q);
   dmf_int8_dequantize_args a = {};
   a.rows = v.rows;
   a.channels = v.k;
