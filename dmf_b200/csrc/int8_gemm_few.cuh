@@ -5,6 +5,10 @@
 // weight.  Each CTA sends the other CTAs their columns of its sums (int32: exact, the order does not matter) through distributed
 // shared memory; after one cluster barrier CTA r adds up columns [r TB / S, (r + 1) TB / S), scales them and writes them, 32
 // consecutive channels of a token per warp instruction.
+//
+// What bounds it: latency.  Of the 4.8 us that 1 x 1152 x 6912 takes, 1.2 are the weight's 8 MB at the HBM's rate; 3.2 us is what 3
+// steps of k take in one tile, and every further step 0.2.  A cluster costs 0.4 to 3 us, so only long sums are split: 16 x 4608 x
+// 1152 takes 10.4 us in one piece and 4.4 in eight.  (Bulk copies between the CTAs instead of stores: 2 us more.)
 #pragma once
 
 #include <type_traits>

@@ -3,7 +3,8 @@
 //   out[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] + bias[n]
 //
 // A block owns 64 x 64 outputs, a thread 4 x 4 of them; 64 bytes of k at a time lie in shared memory as words of four, which
-// dp4a multiplies and adds to int32.  Bytes are read one by one.
+// dp4a multiplies and adds to int32.  Bytes are read one by one.  16384 x 1152 x 3456 takes 1.7 ms here, against 51 us on the tensor
+// cores: rows that this package makes start at multiples of 16 bytes.
 #pragma once
 
 #include <stdint.h>

@@ -106,7 +106,8 @@ class Int8FinalLayer(nn.Module):
 
 def int8_model(model: DMFT) -> DMFT:
     """A copy of a DMFT model on the GPU with its blocks in 8 bits, in eval mode and without gradients; the weights that were
-    quantised are not kept in 16 or 32 bits.  The model must use this package's attention ('fa2' / 'fa3')."""
+    quantised are not kept in 16 or 32 bits.  The model must use this package's attention ('fa2' / 'fa3').  With an fp32 stream the
+    products and the attention give bf16, as under autocast."""
     blocks = list(model.blocks)
     if not all(isinstance(b, DiTBlock) and b.fused for b in blocks):
         raise ValueError("int8_model takes a DMFT model with attn_func 'fa2' or 'fa3'")

@@ -278,6 +278,60 @@ def test_rows_behind_the_last_one_stay_as_they_were():
     assert torch.equal(rows[:40, :100], quantize_int8(src).values)
 
 
+@pytest.mark.parametrize("C,M", [(1152, 2000), (1152, 5), (100, 9), (99, 9), (4608, 1300)])
+def test_the_sum_may_be_written_where_its_term_was(C, M):
+    """the C ABI with sum = residual and sum = x, against results in buffers of their own"""
+    import ctypes
+
+    from dmf_b200 import _lib
+    stream = torch.cuda.current_stream().cuda_stream
+    x, res, w = _randn(M, C, dtype=BF16), _randn(M, C, seed=1), 1 + _randn(C, std=0.1, seed=2)
+    want, total = rms_norm_int8(x, w, residual=res)
+    q, scale = torch.empty(M, -(-C // 16) * 16, dtype=torch.int8, device=DEV), torch.empty(M, device=DEV)
+    a = _lib.Int8RmsNormArgs()
+    a.batch, a.seqlen, a.channels, a.dtype, a.stream_dtype, a.weight_dtype, a.eps = 1, M, C, _lib.INT8_BF16, _lib.INT8_F32, _lib.INT8_F32, 1e-6
+    a.x, a.residual, a.sum = _lib.Rows(x.data_ptr(), 0, C), _lib.Rows(res.data_ptr(), 0, C), _lib.Rows(res.data_ptr(), 0, C)
+    a.weight, a.out, a.stream = w.data_ptr(), _lib.Int8Matrix(q.data_ptr(), q.stride(0), scale.data_ptr()), stream
+    assert _lib.load().dmf_int8_rmsnorm(ctypes.byref(a)) == 0
+    assert torch.equal(res, total) and torch.equal(q[:, :C], want.values) and torch.equal(scale, want.scale)
+    x3, h = x[None].clone(), _randn(1, M, C, dtype=BF16, seed=3)
+    gate, shift, sc = (_randn(1, C, dtype=BF16, seed=s, std=0.3) for s in (4, 5, 6))
+    want, total = ln_modulate_int8(x3, shift, sc, gate=gate, h=h)
+    b = _lib.Int8LnModulateArgs()
+    b.batch, b.seqlen, b.channels, b.eps = 1, M, C, 1e-6
+    b.x, b.h, b.sum = _lib.Rows(x3.data_ptr(), 0, C), _lib.Rows(h.data_ptr(), 0, C), _lib.Rows(x3.data_ptr(), 0, C)
+    b.gate, b.shift, b.scale = (_lib.Mod(t.data_ptr(), 0) for t in (gate, shift, sc))
+    b.out, b.stream = _lib.Int8Matrix(q.data_ptr(), q.stride(0), scale.data_ptr()), stream
+    assert _lib.load().dmf_int8_ln_modulate(ctypes.byref(b)) == 0
+    assert torch.equal(x3, total) and torch.equal(q[:, :C], want.values[0]) and torch.equal(scale, want.scale[0])
+
+
+def test_more_than_2_to_the_31_elements():
+    M, C, tail = 600_000, 4096, 700                    # 2.46e9 elements
+    row = _randn(1000, C, dtype=BF16)
+    x = row.repeat(M // 1000, 1)
+    x[-tail:] = _randn(tail, C, dtype=BF16, seed=9)
+    w, bias = quantize_int8(_randn(24, C, seed=2)), _randn(24)
+    for act in (None, "gelu"):
+        rows = quantize_int8(x, act)
+        end = quantize_int8(x[-tail:], act)
+        assert torch.equal(rows.values[-tail:], end.values) and torch.equal(rows.scale[-tail:], end.scale)
+    assert torch.equal(rows.dequantize()[-tail:], end.dequantize())
+    out = int8_linear(rows, w, bias)
+    assert torch.equal(out[-tail:], int8_linear(end, w, bias)) and torch.equal(out[:1000], out[1000:2000])
+    ones = torch.ones(C, device=DEV)
+    rows, z = rms_norm_int8(x, ones, residual=x)
+    end, z_end = rms_norm_int8(x[-tail:], ones, residual=x[-tail:])
+    assert torch.equal(rows.values[-tail:], end.values) and torch.equal(z[-tail:], z_end)
+    del rows, z, out
+    mod = _randn(2, 6 * C, dtype=BF16, std=0.2)
+    g, sh, sc = mod.chunk(6, -1)[2:5]
+    x3 = x.view(2, M // 2, C)
+    rows, z = ln_modulate_int8(x3, sh, sc, gate=g, h=x3)
+    end, z_end = ln_modulate_int8(x3[1:, -tail:], sh[1:], sc[1:], gate=g[1:], h=x3[1:, -tail:])
+    assert torch.equal(rows.values[1, -tail:], end.values[0]) and torch.equal(z[1, -tail:], z_end[0])
+
+
 def test_a_block_half_as_it_is_used():
     """adaLN, first product, GELU, second product, gate: the ops one after the other against the same steps in fp64 on their own
     8-bit operands, and against the layer in fp64 with the error that 8 bits have"""
@@ -367,6 +421,17 @@ def test_refusals_of_gradients_and_tangents():
     # an input of a transform that carries no tangent of its own
     y, _ = torch.func.jvp(lambda t: t * quantize_int8(x.detach()).scale[:, None], (x.detach(),), (x.detach(),))
     assert torch.equal(y, x.detach() * quantize_int8(x.detach()).scale[:, None])
+
+
+def test_traced_and_under_other_transforms():
+    w = quantize_int8(_randn(48, 100))
+    x, y = _randn(6, 100, dtype=BF16), _randn(6, 100, dtype=BF16, seed=1)
+    f = lambda t: int8_linear(quantize_int8(t), w)
+    assert torch.equal(torch.jit.trace(f, (x,))(y), f(y))
+    with pytest.raises(Exception):
+        torch.func.vmap(f)(x[None])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: quantize_int8(t).scale.sum())(x.float())
 
 
 def test_compiled():
