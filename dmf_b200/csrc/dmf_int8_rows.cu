@@ -137,6 +137,9 @@ int launch_rows(const Int8RowParams& p, cudaStream_t stream) {
     }
     if (st != kNoKernel) return st;
   }
+  if (p.channels <= 1024 * kSingles)
+    return launch_dependent(int8_row_single_kernel<kOp>, dim3(static_cast<unsigned>(p.rows)),
+                            ((p.channels + kSingles - 1) / kSingles + 31) / 32 * 32, 0, 1, stream, p);
   return launch_dependent(int8_row_any_kernel<kOp>, dim3(static_cast<unsigned>(p.rows)), kRowThreads, 0, 1, stream, p);
 }
 

@@ -270,13 +270,26 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
               tma_store_commit();
             }
           } else {
+            // rows that start anywhere: a row at a time, 32 bits per lane; in rows that start between two words the words are
+            // put together from two lanes'
             __syncwarp();
-#pragma unroll 1
-            for (int i = lane; i < 32 * kWide; i += 32) {
-              const int row = i / kWide, c = i % kWide;
-              if (m0 + row < p.m && n + c < p.n)
-                static_cast<T*>(p.out)[(static_cast<int64_t>(m0) + row) * p.out_stride + n + c] =
-                    *reinterpret_cast<const T*>(stage + slot(row, c * static_cast<int>(sizeof(T)) / 16) + c * static_cast<int>(sizeof(T)) % 16);
+            const int rows = min(32, p.m - m0), cols = min(kWide, p.n - n);
+            T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(m0) * p.out_stride + n;
+#pragma unroll 4
+            for (int row = 0; row < rows; ++row, dst += p.out_stride) {
+              const uint32_t v = *reinterpret_cast<const uint32_t*>(stage + slot(row, lane >> 2) + (lane & 3) * 4);
+              if constexpr (sizeof(T) == 4) {
+                if (lane < cols) *reinterpret_cast<uint32_t*>(dst + lane) = v;
+              } else {
+                uint16_t* d = reinterpret_cast<uint16_t*>(dst);
+                const uint32_t odd = reinterpret_cast<uintptr_t>(dst) >> 1 & 1u;   // (the whole warp alike)
+                const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
+                const int c = 2 * lane + static_cast<int>(odd);
+                const uint32_t u = odd != 0u ? __funnelshift_r(v, next, 16) : v;
+                if (odd != 0u && lane == 0 && cols > 0) d[0] = static_cast<uint16_t>(v);
+                if (c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = u;
+                else if (c < cols) d[c] = static_cast<uint16_t>(u);
+              }
             }
           }
           __syncwarp();

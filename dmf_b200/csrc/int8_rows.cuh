@@ -7,8 +7,9 @@
 // int8_row_block_kernel has a block per row: few rows, where latency counts, and wide ones without a sample's vectors, where
 // blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 45 us
 // against 51, with GELU 66 against 78; gated LayerNorm 189 against 133).  Both move 16 bytes at a time.
-// int8_row_any_kernel takes what these do not: odd widths, strides and alignments, mixed 16-bit types, rows beyond 16384
-// channels.  Sums and the arithmetic are fp32.
+// int8_row_single_kernel takes what these do not - odd widths, strides and alignments, mixed 16-bit types - in the same way, an
+// element at a time, and int8_row_any_kernel what is then too wide for a block's registers, computing the row again from global
+// memory in every pass.  Sums and the arithmetic are fp32.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -403,6 +404,68 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
           for (int i = 0; i < 8; ++i) f[i] += 1.f;
         }
       });
+}
+
+// A block per row, eight single elements per thread: c = thread + k * threads.
+constexpr int kSingles = 8;
+template <int kOp>
+__global__ void __launch_bounds__(1024) int8_row_single_kernel(const Int8RowParams p) {
+  __shared__ float red[2][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int turn = 0;
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / p.seqlen, l = row % p.seqlen;
+  const int t = threadIdx.x, threads = blockDim.x;
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int k = 0; k < kSingles; ++k)
+      if (t + k * threads < p.channels) f(k, t + k * threads);
+  };
+  auto load = [&](const void* src, int dtype, int64_t at, float (&f)[kSingles]) {   // the type decided once, so that loads overlap
+    if (dtype == 0) each([&](int k, int c) { f[k] = row_load(src, 0, at + c); });
+    else if (dtype == 1) each([&](int k, int c) { f[k] = row_load(src, 1, at + c); });
+    else each([&](int k, int c) { f[k] = row_load(src, 2, at + c); });
+  };
+  float z[kSingles] = {}, v[kSingles] = {}, w[kSingles] = {};
+  load(p.x, p.x_dtype, b * p.x_sb + l * p.x_sl, z);
+  if constexpr (kIsNorm<kOp>) {
+    if (p.add != nullptr) {
+      load(p.add, p.add_dtype, b * p.add_sb + l * p.add_sl, v);
+      if constexpr (kOp == kRowLn) load(p.gate, p.mod_dtype, b * p.gate_sb, w);
+      each([&](int k, int) { z[k] = kOp == kRowLn ? fmaf(w[k], v[k], z[k]) : v[k] + z[k]; });
+      const int64_t sum0 = b * p.sum_sb + l * p.sum_sl;
+      if (p.sum_dtype == 0) each([&](int k, int c) { row_store(p.sum, 0, sum0 + c, z[k]); });
+      else if (p.sum_dtype == 1) each([&](int k, int c) { row_store(p.sum, 1, sum0 + c, z[k]); });
+      else each([&](int k, int c) { row_store(p.sum, 2, sum0 + c, z[k]); });
+    }
+    if constexpr (kOp == kRowLn) {
+      load(p.scale, p.mod_dtype, b * p.scale_sb, w);
+      load(p.shift, p.mod_dtype, b * p.shift_sb, v);
+    } else {
+      load(p.weight, p.mod_dtype, 0, w);
+    }
+    const float inv_c = 1.f / static_cast<float>(p.channels);
+    if constexpr (kOp == kRowLn) {
+      float s = 0.f;
+      each([&](int k, int) { s += z[k]; });
+      const float mean = row_block_sum(s, red, turn) * inv_c;
+      each([&](int k, int) { z[k] -= mean; });
+    }
+    float s = 0.f;
+    each([&](int k, int) { s = fmaf(z[k], z[k], s); });
+    const float r = rsqrtf(row_block_sum(s, red, turn) * inv_c + p.eps);
+    each([&](int k, int) { z[k] = kOp == kRowLn ? fmaf(z[k] * r, 1.f + w[k], v[k]) : z[k] * r * w[k]; });
+  } else {
+    each([&](int k, int) { z[k] = row_act<kActOf<kOp>>(z[k]); });
+  }
+  float top = 0.f;
+  each([&](int k, int) { top = row_max3(top, z[k], z[k]); });
+  const RowScale rs = row_scale_of(row_block_max(__float_as_uint(top), red, turn));
+  const bool zeros = rs.inverse == 0.f;
+  int8_t* q = p.q + row * p.q_stride;
+  each([&](int k, int c) { q[c] = static_cast<int8_t>(zeros ? 0u : row_quantize(z[k], rs.inverse) & 0xffu); });
+  if (t == 0) p.row_scale[row] = rs.scale;
 }
 
 template <int kOp>

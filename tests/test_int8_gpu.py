@@ -307,7 +307,7 @@ def test_the_sum_may_be_written_where_its_term_was(C, M):
 
 
 def test_more_than_2_to_the_31_elements():
-    M, C, tail = 600_000, 4096, 700                    # 2.46e9 elements
+    M, C, tail = 600_000, 4096, 1300                   # 2.46e9 elements; the end alone takes the same kernels
     row = _randn(1000, C, dtype=BF16)
     x = row.repeat(M // 1000, 1)
     x[-tail:] = _randn(tail, C, dtype=BF16, seed=9)
@@ -428,8 +428,8 @@ def test_traced_and_under_other_transforms():
     x, y = _randn(6, 100, dtype=BF16), _randn(6, 100, dtype=BF16, seed=1)
     f = lambda t: int8_linear(quantize_int8(t), w)
     assert torch.equal(torch.jit.trace(f, (x,))(y), f(y))
-    with pytest.raises(Exception):
-        torch.func.vmap(f)(x[None])
+    both = torch.stack([x, y])
+    assert torch.equal(torch.func.vmap(f)(both), torch.stack([f(x), f(y)]))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: quantize_int8(t).scale.sum())(x.float())
 
