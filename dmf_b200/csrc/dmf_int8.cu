@@ -63,7 +63,7 @@ int launch_pair_gemm(const Int8GemmParams& p, int sms, cudaStream_t stream) {
   static bool allowed[64];
   const auto kernel = int8_gemm_pair_kernel<BN, T>;
   if (!allow_smem(kernel, Int8PairTraits<BN>::kSmemBytes, allowed)) return DMF_ATTN_ERR_LAUNCH;
-  const int tiles = p.tiles_m * p.tiles_n, clusters = tiles < sms / 2 ? tiles : sms / 2;
+  const int tiles = p.tiles_m * (p.tiles_n + p.narrow), clusters = tiles < sms / 2 ? tiles : sms / 2;
   return launch_dependent(kernel, dim3(2u * clusters), Int8PairTraits<BN>::kThreads, Int8PairTraits<BN>::kSmemBytes, 2, stream, p);
 }
 
@@ -75,6 +75,9 @@ int launch_few_gemm(const Int8GemmParams& p, int splits, cudaStream_t stream) {
   return launch_dependent(kernel, dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * splits)), kInt8FewThreads, Int8FewTraits<TB>::kSmemBytes,
                         splits, stream, p, splits);
 }
+
+// Whether the columns of a product on CTA pairs end in tiles of half the width.
+bool narrow_end(int n, int bn) { return bn == 256 && n % 256 != 0 && n % 256 <= 128; }
 
 // How a product is cut up: on CTA pairs with tiles of 256 x bn, or (few) tiles of tb tokens x 128 channels, k over `splits` CTAs.
 struct GemmPlan {
@@ -105,7 +108,7 @@ GemmPlan plan_gemm(int m, int n, int k, int sms) {
   };
   struct { int bn; double c, t; } pairs[] = {{128, 0.35, 0.256}, {192, 0.77, 0.279}, {256, 0.95, 0.33}};
   for (const auto& g : pairs) {
-    const double rounds = tiles(256, g.bn) / (sms / 2);
+    const double rounds = (tiles(256, g.bn) - (narrow_end(n, g.bn) ? 0.4 * tiles(256, n) : 0.0)) / (sms / 2);
     consider(false, g.bn, 1, 3.4 + (std::fmax(rounds, 1.0) + std::ceil(rounds)) / 2 * (g.c + steps * g.t));
   }
   struct { int tb; double e; } fews[] = {{16, 0.55}, {32, 1.4}, {64, 3.2}};
@@ -151,8 +154,10 @@ int run_plan(const GemmPlan& g, const dmf_int8_linear_args* a, int sms) {
   const int64_t tiles_m = (static_cast<int64_t>(a->m) + (g.few ? g.tile : 256) - 1) / (g.few ? g.tile : 256);
   const int64_t tiles_n = (static_cast<int64_t>(a->n) + (g.few ? 128 : g.tile) - 1) / (g.few ? 128 : g.tile);
   if (tiles_m * tiles_n * g.splits > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;
+  p.narrow = !g.few && narrow_end(a->n, g.tile);
+  if (p.narrow && (st = make_map8(&p.w_half_map, a->w, a->n, a->k, 64)) != DMF_ATTN_OK) return st;
   p.tiles_m = static_cast<int>(tiles_m);
-  p.tiles_n = static_cast<int>(tiles_n);
+  p.tiles_n = static_cast<int>(tiles_n) - p.narrow;
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   switch (a->out_dtype) {
     case DMF_INT8_BF16: return launch_gemm<__nv_bfloat16>(g, p, sms, stream);

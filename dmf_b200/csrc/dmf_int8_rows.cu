@@ -56,6 +56,19 @@ int blocks_per_sm(int registers, int threads, int smem) {
   return blocks > 1 ? blocks : 1;
 }
 
+// A kernel's registers per thread, asked for once.
+template <typename Kernel>
+int registers_of(Kernel kernel, std::atomic<int>& registers) {
+  if (registers.load(std::memory_order_relaxed) != 0) return DMF_ATTN_OK;
+  cudaFuncAttributes attr;
+  if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return DMF_ATTN_ERR_LAUNCH;
+  }
+  registers.store(attr.numRegs, std::memory_order_relaxed);
+  return DMF_ATTN_OK;
+}
+
 constexpr int kWarpRowEights = 160;            // a warp's registers hold rows of up to 5 x 32 eights
 constexpr int kMaxEights = 4 * kGroupThreads;  // a block's: 4 per thread
 
@@ -73,14 +86,8 @@ int launch_group(const Int8RowParams& p, int threads, int sms, cudaStream_t stre
   const int smem = kRowVectors<kOp, TA> * p.channels * 4;
   if (smem > 48 * 1024 && !allow_smem(kernel, kRowVectors<kOp, TA> * kMaxEights * 32, allowed)) return DMF_ATTN_ERR_LAUNCH;
   static std::atomic<int> registers{0};
-  if (registers.load(std::memory_order_relaxed) == 0) {
-    cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return DMF_ATTN_ERR_LAUNCH;
-    }
-    registers.store(attr.numRegs, std::memory_order_relaxed);
-  }
+  const int st = registers_of(kernel, registers);
+  if (st != DMF_ATTN_OK) return st;
   // one wave: as many blocks as the SMs hold at a time, cut at the samples' ends
   const int64_t samples = kOp == kRowLn ? p.batch : 1, per_sample = kOp == kRowLn ? p.seqlen : p.rows, unit = kWarp ? kRowThreads / 32 : 1;
   const int64_t resident = static_cast<int64_t>(sms) * blocks_per_sm(registers.load(std::memory_order_relaxed), threads, smem);
@@ -137,9 +144,15 @@ int launch_rows(const Int8RowParams& p, cudaStream_t stream) {
     }
     if (st != kNoKernel) return st;
   }
-  if (p.channels <= 1024 * kSingles)
-    return launch_dependent(int8_row_single_kernel<kOp>, dim3(static_cast<unsigned>(p.rows)),
-                            ((p.channels + kSingles - 1) / kSingles + 31) / 32 * 32, 0, 1, stream, p);
+  auto singles = [&](auto kernel, int warps) {
+    return launch_dependent(kernel, dim3(static_cast<unsigned>((p.rows * warps + 7) / 8)), kRowThreads, 0, 1, stream, p);
+  };
+  if (p.channels <= 512) return singles(int8_row_single_kernel<kOp, 16, 1>, 1);
+  if (p.channels <= 1024) return singles(int8_row_single_kernel<kOp, 32, 1>, 1);
+  if (p.channels <= 1536) return singles(int8_row_single_kernel<kOp, 24, 2>, 2);
+  if (p.channels <= 2048) return singles(int8_row_single_kernel<kOp, 32, 2>, 2);
+  if (p.channels <= 4096) return singles(int8_row_single_kernel<kOp, 32, 4>, 4);
+  if (p.channels <= 8192) return singles(int8_row_single_kernel<kOp, 32, 8>, 8);
   return launch_dependent(int8_row_any_kernel<kOp>, dim3(static_cast<unsigned>(p.rows)), kRowThreads, 0, 1, stream, p);
 }
 
@@ -245,16 +258,18 @@ int run_dequantize(const dmf_int8_dequantize_args* a) {
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   const bool vectors = a->channels % 8 == 0 && reinterpret_cast<uintptr_t>(a->x.values) % 8 == 0 && (a->rows == 1 || a->x.stride % 8 == 0) &&
                        whole_vectors(a->out, a->out_dtype, 0, 1, a->out_stride, a->rows == 1 ? 1 : 2);
-  if (!vectors)
-    return launch_dependent(int8_dequantize_any_kernel, dim3(static_cast<unsigned>(a->rows)), kRowThreads, 0, 1, stream,
-                            static_cast<const int8_t*>(a->x.values), a->x.stride, static_cast<const float*>(a->x.scale), a->out, a->out_stride,
-                            a->out_dtype, a->channels);
-  const int eights = a->channels / 8, pieces = (eights + kDequantizeEights - 1) / kDequantizeEights;
+  const int per_piece = vectors ? 8 * kDequantizeEights : kDequantizeSingles, pieces = (a->channels + per_piece - 1) / per_piece;
   const int64_t blocks = (a->rows * pieces + kRowThreads / 32 - 1) / (kRowThreads / 32);
   if (blocks > 0x7fffffff) return DMF_ATTN_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int8_t* values = a->x.values;
+  const float* scale = a->x.scale;
+  if (!vectors)
+    return launch_dependent(int8_dequantize_any_kernel, grid, kRowThreads, 0, 1, stream, values, a->x.stride, scale, a->out, a->out_stride,
+                            a->out_dtype, a->rows, a->channels, pieces);
   auto launch = [&](auto kernel) {
-    return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, 1, stream, static_cast<const int8_t*>(a->x.values),
-                            a->x.stride, static_cast<const float*>(a->x.scale), a->out, a->out_stride, a->rows, eights, pieces);
+    return launch_dependent(kernel, grid, kRowThreads, 0, 1, stream, values, a->x.stride, scale, a->out, a->out_stride, a->rows,
+                            a->channels / 8, pieces);
   };
   switch (a->out_dtype) {
     case DMF_INT8_BF16: return launch(int8_dequantize_kernel<__nv_bfloat16>);

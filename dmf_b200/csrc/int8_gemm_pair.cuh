@@ -6,6 +6,8 @@
 // M = 256, N = BN, 32 bytes of k each.  CTA r holds 128 of the tile's rows of x and half of its rows of w, so a 128-byte step of
 // k costs each SM 16 KB + BN / 2 * 128 bytes of loads for 256 x BN x 128 products of the pair.
 //
+// With BN = 256 a last stretch of at most 128 columns is done in tiles of half the width (N = 1152: 4.5 tiles a row instead of 5).
+//
 // Warps: 0 TMA producer (both CTAs), 1 MMA issuer (leader CTA), 2.. epilogue (both CTAs).  Two accumulators of BN columns
 // alternate in tensor memory, so the epilogue of a tile runs under the products of the next one.  An epilogue warp takes 32 rows
 // (its quarter of the lanes) and 64 or 128 columns, 64 at a time; the rounded results go through 4 KB of its own to a TMA store.
@@ -34,6 +36,7 @@ namespace dmf {
 
 struct Int8GemmParams {
   CUtensorMap x_map, w_map;     // boxes of 128 bytes of k; x: 128 rows (pair) / the tile's tokens, w: BN / 2 rows (pair) / 128
+  CUtensorMap w_half_map;       // pair, narrow: boxes of 64 rows of w
   CUtensorMap out_map;          // pair, out_vec: boxes of 128 bytes x 32 rows
   const float *x_scale, *w_scale;
   const void* bias;
@@ -41,7 +44,8 @@ struct Int8GemmParams {
   int32_t* status_word;
   int64_t out_stride;
   int m, n, k;
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n;         // pair: without the narrow ones
+  int narrow;                   // pair: the columns end in tiles of half the width
   int out_dtype, bias_dtype;
   int out_vec;                  // rows of out start at multiples of 16 bytes
 };
@@ -74,13 +78,35 @@ struct Int8PairTraits {
 
 constexpr int kInt8GroupM = 8;   // tiles run over w within groups of 8 row tiles: w is read from HBM once per 2048 rows at most
 
-__device__ __forceinline__ void int8_tile(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int per_group = kInt8GroupM * tiles_n;
-  const int g = t / per_group, r = t % per_group;
-  const int rows = min(kInt8GroupM, tiles_m - g * kInt8GroupM);
-  tm = g * kInt8GroupM + r % rows;
-  tn = r / rows;
-}
+// The tiles of a cluster, in order: its share of the whole tiles, then of the narrow ones (the last 128 columns or fewer), which
+// go to the clusters that had one whole tile less, twice, before everybody gets them in turn.
+struct Int8TileWalk {
+  int whole, tiles_m, tiles_n, narrow, clusters, id;
+  int t, turn;
+  __device__ __forceinline__ Int8TileWalk(const Int8GemmParams& p, int id_, int clusters_)
+      : whole(p.tiles_m * p.tiles_n), tiles_m(p.tiles_m), tiles_n(p.tiles_n), narrow(p.narrow ? p.tiles_m : 0), clusters(clusters_), id(id_),
+        t(id_), turn(id_ >= whole % clusters_ ? 0 : 2) {}
+  // the next tile, false after the last
+  __device__ __forceinline__ bool next(int& tm, int& tn, bool& is_narrow) {
+    if (t < whole) {
+      const int per_group = kInt8GroupM * tiles_n;
+      const int g = t / per_group, r = t % per_group;
+      const int rows = min(kInt8GroupM, tiles_m - g * kInt8GroupM);
+      tm = g * kInt8GroupM + r % rows;
+      tn = r / rows;
+      is_narrow = false;
+      t += clusters;
+      return true;
+    }
+    const int busy = whole % clusters, free = clusters - busy;
+    const int slot = turn < 2 ? turn * free + id - busy : 2 * free + id + (turn - 2) * clusters;
+    ++turn;
+    tm = slot;
+    tn = tiles_n;
+    is_narrow = true;
+    return slot < narrow;
+  }
+};
 
 template <int BN, typename T>
 __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pair_kernel(const __grid_constant__ Int8GemmParams p) {
@@ -100,7 +126,8 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
-  const int tiles = p.tiles_m * p.tiles_n, k_steps = (p.k + 127) >> 7;
+  const int k_steps = (p.k + 127) >> 7;
+  Int8TileWalk walk(p, cluster_id, num_clusters);
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -132,18 +159,18 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
       prefetch_tensor_map(&p.w_map);
       uint32_t cnt = 0;
       bool ok = true;
-      for (int t = cluster_id; ok && t < tiles; t += num_clusters) {
-        int tm, tn;
-        int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
-        const int x_row = tm * 256 + static_cast<int>(rank) * 128, w_row = tn * BN + static_cast<int>(rank) * (BN / 2);
+      int tm, tn;
+      bool narrow;
+      while (ok && walk.next(tm, tn, narrow)) {
+        const int x_row = tm * 256 + static_cast<int>(rank) * 128, w_row = tn * BN + static_cast<int>(rank) * (narrow ? 64 : BN / 2);
         for (int kk = 0; kk < k_steps; ++kk, ++cnt) {
           const uint32_t s = cnt % TR::kStages, ph = (cnt / TR::kStages) & 1u;
           ok = mbar_wait(bar(TR::kBarEmpty + s), ph ^ 1u, abort_flag, p.status_word, kRoleInt8Producer + TR::kBarEmpty + s);
           if (!ok) break;
           const uint32_t dst = s_ring + s * TR::kStageBytes, fb = lbar(TR::kBarFull + s);
-          mbar_arrive_expect_tx_cluster(fb, TR::kStageBytes);
+          mbar_arrive_expect_tx_cluster(fb, narrow ? TR::kXBytes + 64 * 128 : TR::kStageBytes);
           tma_load_2d_pair(dst, &p.x_map, fb, kk * 128, x_row);
-          tma_load_2d_pair(dst + TR::kXBytes, &p.w_map, fb, kk * 128, w_row);
+          tma_load_2d_pair(dst + TR::kXBytes, narrow ? &p.w_half_map : &p.w_map, fb, kk * 128, w_row);
         }
       }
     }
@@ -151,11 +178,11 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
     // ===================== MMA issuer (leader CTA only) =======================
     if (rank == 0) {
       const bool leader = elect_one();
-      constexpr uint32_t idesc = make_idesc_i8(256, BN);
       uint32_t cnt = 0, tcnt = 0;
-      bool ok = true;
-      for (int t = cluster_id; ok && t < tiles; t += num_clusters, ++tcnt) {
-        const uint32_t a = tcnt & 1u;
+      bool ok = true, narrow;
+      int tm, tn;
+      for (; ok && walk.next(tm, tn, narrow); ++tcnt) {
+        const uint32_t a = tcnt & 1u, idesc = narrow ? make_idesc_i8(256, 128) : make_idesc_i8(256, BN);
         // the epilogue of the tile before the last has read this accumulator (both CTAs)
         ok = mbar_wait(bar(TR::kBarAccEmpty + a), ((tcnt >> 1) & 1u) ^ 1u, abort_flag, p.status_word,
                        kRoleInt8Mma + TR::kBarAccEmpty + a);
@@ -190,28 +217,29 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
     const int frow = lane >> 2, fcol = 2 * (lane & 3);  // this lane's first row and column of a fragment
     // scales and bias of a tile's columns and the scales of this lane's rows: in registers a tile ahead
     float next_w[kPer], next_b[kPer], next_x[4];
-    auto fetch = [&](int t) {
-      if (t >= tiles) return;
-      int tm, tn;
-      int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
+    int tm, tn, next_tm, next_tn;
+    bool narrow, next_narrow, more;
+    auto fetch = [&] {
+      more = walk.next(next_tm, next_tn, next_narrow);
+      if (!more) return;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int n = tn * BN + col0 + i * 32 + lane;
+        const int n = next_tn * BN + col0 + i * 32 + lane;
         next_w[i] = n < p.n ? p.w_scale[n] : 0.f;
         next_b[i] = n < p.n && p.bias != nullptr ? row_load(p.bias, p.bias_dtype, n) : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t m = static_cast<int64_t>(tm) * 256 + rank * 128 + quarter * 32 + frow + 8 * i;
+        const int64_t m = static_cast<int64_t>(next_tm) * 256 + rank * 128 + quarter * 32 + frow + 8 * i;
         next_x[i] = m < p.m ? p.x_scale[m] : 0.f;
       }
     };
     auto slot = [](int row, int piece) -> int { return row * 128 + ((piece ^ (row & 7)) << 4); };   // the store map's swizzle
-    fetch(cluster_id);
-    uint32_t tcnt = 0;
-    for (int t = cluster_id; t < tiles; t += num_clusters, ++tcnt) {
-      int tm, tn;
-      int8_tile(t, p.tiles_m, p.tiles_n, tm, tn);
+    fetch();
+    for (uint32_t tcnt = 0; more; ++tcnt) {
+      tm = next_tm;
+      tn = next_tn;
+      narrow = next_narrow;
       const int n0 = tn * BN + col0;
       const int m0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
       const uint32_t a = tcnt & 1u;
@@ -221,12 +249,16 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
         s_w[i * 32 + lane] = next_w[i];
         s_b[i * 32 + lane] = next_b[i];
       }
-      fetch(t + num_clusters);
+      fetch();
       __syncwarp();
       const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(TR::kBarAccFull + a), (tcnt >> 1) & 1u, abort_flag, p.status_word,
                                                         kRoleInt8Epilogue + TR::kBarAccFull + a));
       if (!ok) break;
       tc_fence_after_sync();
+      if (narrow && col0 >= 128) {                     // no columns of this warp's
+        mbar_arrive_warp_cluster(lbar(TR::kBarAccEmpty + a));
+        continue;
+      }
 #pragma unroll
       for (int c0 = 0; c0 < kCols; c0 += 32) {
         uint32_t lo[16], hi[16];                       // rows frow, + 8 and + 16, + 24
@@ -275,20 +307,26 @@ __global__ void __launch_bounds__(Int8PairTraits<BN>::kThreads, 1) int8_gemm_pai
             __syncwarp();
             const int rows = min(32, p.m - m0), cols = min(kWide, p.n - n);
             T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(m0) * p.out_stride + n;
-#pragma unroll 4
-            for (int row = 0; row < rows; ++row, dst += p.out_stride) {
-              const uint32_t v = *reinterpret_cast<const uint32_t*>(stage + slot(row, lane >> 2) + (lane & 3) * 4);
-              if constexpr (sizeof(T) == 4) {
-                if (lane < cols) *reinterpret_cast<uint32_t*>(dst + lane) = v;
-              } else {
-                uint16_t* d = reinterpret_cast<uint16_t*>(dst);
-                const uint32_t odd = reinterpret_cast<uintptr_t>(dst) >> 1 & 1u;   // (the whole warp alike)
-                const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
-                const int c = 2 * lane + static_cast<int>(odd);
-                const uint32_t u = odd != 0u ? __funnelshift_r(v, next, 16) : v;
-                if (odd != 0u && lane == 0 && cols > 0) d[0] = static_cast<uint16_t>(v);
-                if (c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = u;
-                else if (c < cols) d[c] = static_cast<uint16_t>(u);
+#pragma unroll 1
+            for (int row0 = 0; row0 < rows; row0 += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const uint32_t*>(stage + slot(row0 + i, lane >> 2) + (lane & 3) * 4);
+#pragma unroll
+              for (int i = 0; i < 8; ++i, dst += p.out_stride) {
+                if (row0 + i >= rows) break;
+                if constexpr (sizeof(T) == 4) {
+                  if (lane < cols) *reinterpret_cast<uint32_t*>(dst + lane) = v[i];
+                } else {
+                  uint16_t* d = reinterpret_cast<uint16_t*>(dst);
+                  const uint32_t odd = reinterpret_cast<uintptr_t>(dst) >> 1 & 1u;   // (the whole warp alike)
+                  const uint32_t next = __shfl_down_sync(0xffffffffu, v[i], 1);
+                  const int c = 2 * lane + static_cast<int>(odd);
+                  const uint32_t u = odd != 0u ? __funnelshift_r(v[i], next, 16) : v[i];
+                  if (odd != 0u && lane == 0 && cols > 0) d[0] = static_cast<uint16_t>(v[i]);
+                  if (c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = u;
+                  else if (c < cols) d[c] = static_cast<uint16_t>(u);
+                }
               }
             }
           }

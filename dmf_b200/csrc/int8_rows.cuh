@@ -362,14 +362,16 @@ __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_
   constexpr int kStep = kWarp ? kRowThreads / 32 : 1;
   RowLoads<kOp, TX, TA, NV> loads;
   auto start = [&](int64_t l) {
-    const int64_t b = kOp == kRowLn ? b0 : l / p.seqlen, i = kOp == kRowLn ? l : l % p.seqlen;
+    const int64_t b = kOp == kRowLn ? b0 : static_cast<unsigned>(l) / static_cast<unsigned>(p.seqlen);   // rows fit in 31 bits
+    const int64_t i = kOp == kRowLn ? l : static_cast<unsigned>(l) % static_cast<unsigned>(p.seqlen);
     loads.start(p, b * p.x_sb + i * p.x_sl, b * p.add_sb + i * p.add_sl, t, threads);
   };
   int turn = 0;
   int64_t l = l0 + (kWarp ? threadIdx.x >> 5 : 0);
   if (l < l1) start(l);
   for (; l < l1; l += kStep) {
-    const int64_t b = kOp == kRowLn ? b0 : l / p.seqlen, i = kOp == kRowLn ? l : l % p.seqlen;
+    const int64_t b = kOp == kRowLn ? b0 : static_cast<unsigned>(l) / static_cast<unsigned>(p.seqlen);   // rows fit in 31 bits
+    const int64_t i = kOp == kRowLn ? l : static_cast<unsigned>(l) % static_cast<unsigned>(p.seqlen);
     row_in_registers<kOp, TX, TA, NV>(
         p, loads, b0 * per_sample + l, b * p.x_sb + i * p.x_sl, b * p.sum_sb + i * p.sum_sl, t, threads,
         [&] {
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
   grid_launch_dependents();
   int turn = 0;
   const int64_t row = blockIdx.x;
-  const int64_t b = row / p.seqlen, l = row % p.seqlen;
+  const int64_t b = blockIdx.x / static_cast<unsigned>(p.seqlen), l = blockIdx.x % static_cast<unsigned>(p.seqlen);
   RowLoads<kOp, TX, TA, NV> loads;
   loads.start(p, b * p.x_sb + l * p.x_sl, b * p.add_sb + l * p.add_sl, threadIdx.x, blockDim.x);
   row_in_registers<kOp, TX, TA, NV>(
@@ -406,65 +408,110 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
       });
 }
 
-// A block per row, eight single elements per thread: c = thread + k * threads.
-constexpr int kSingles = 8;
-template <int kOp>
-__global__ void __launch_bounds__(1024) int8_row_single_kernel(const Int8RowParams p) {
-  __shared__ float red[2][32];
+// Rows that cannot be read as vectors: kWarps warps on a row, NE single elements per lane, c = thread of the row + k * threads; a
+// block of eight warps has 8 / kWarps rows.  Bound by instruction issue (a load and a store for every element): quantisation of
+// 11136 x 1919 22 us, of 1920 in vectors 13, residual + RMS norm 52 and 26, gated LayerNorm 84 and 35; a block per row took 37, 70 and
+// 130, its barriers and divisions not spread over enough elements.
+template <int kOp, int NE, int kWarps>
+__global__ void __launch_bounds__(kRowThreads) int8_row_single_kernel(const Int8RowParams p) {
+  constexpr int kThreads = 32 * kWarps;
+  __shared__ float red[kRowThreads / 32];
   grid_dependency_wait();
   grid_launch_dependents();
-  int turn = 0;
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / p.seqlen, l = row % p.seqlen;
-  const int t = threadIdx.x, threads = blockDim.x;
-  auto each = [&](auto&& f) {
+  const int t = threadIdx.x % kThreads, group = threadIdx.x / kThreads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (8 / kWarps) + group;
+  if (row >= p.rows) return;                           // (a group's warps alike: its barriers are its own)
+  const int64_t b = static_cast<unsigned>(row) / static_cast<unsigned>(p.seqlen), l = static_cast<unsigned>(row) % static_cast<unsigned>(p.seqlen);
+  auto up = [&](auto&& within, auto&& across, float v) -> float {   // over the row's threads
+    v = within(v);
+    if constexpr (kWarps > 1) {
+      named_bar_sync(1 + group, kThreads);             // the last reduction has been read
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+      named_bar_sync(1 + group, kThreads);
+      v = red[group * kWarps];
 #pragma unroll
-    for (int k = 0; k < kSingles; ++k)
-      if (t + k * threads < p.channels) f(k, t + k * threads);
-  };
-  auto load = [&](const void* src, int dtype, int64_t at, float (&f)[kSingles]) {   // the type decided once, so that loads overlap
-    if (dtype == 0) each([&](int k, int c) { f[k] = row_load(src, 0, at + c); });
-    else if (dtype == 1) each([&](int k, int c) { f[k] = row_load(src, 1, at + c); });
-    else each([&](int k, int c) { f[k] = row_load(src, 2, at + c); });
-  };
-  float z[kSingles] = {}, v[kSingles] = {}, w[kSingles] = {};
-  load(p.x, p.x_dtype, b * p.x_sb + l * p.x_sl, z);
-  if constexpr (kIsNorm<kOp>) {
-    if (p.add != nullptr) {
-      load(p.add, p.add_dtype, b * p.add_sb + l * p.add_sl, v);
-      if constexpr (kOp == kRowLn) load(p.gate, p.mod_dtype, b * p.gate_sb, w);
-      each([&](int k, int) { z[k] = kOp == kRowLn ? fmaf(w[k], v[k], z[k]) : v[k] + z[k]; });
-      const int64_t sum0 = b * p.sum_sb + l * p.sum_sl;
-      if (p.sum_dtype == 0) each([&](int k, int c) { row_store(p.sum, 0, sum0 + c, z[k]); });
-      else if (p.sum_dtype == 1) each([&](int k, int c) { row_store(p.sum, 1, sum0 + c, z[k]); });
-      else each([&](int k, int c) { row_store(p.sum, 2, sum0 + c, z[k]); });
+      for (int w = 1; w < kWarps; ++w) v = across(v, red[group * kWarps + w]);
     }
-    if constexpr (kOp == kRowLn) {
-      load(p.scale, p.mod_dtype, b * p.scale_sb, w);
-      load(p.shift, p.mod_dtype, b * p.shift_sb, v);
+    return v;
+  };
+  auto sum_up = [&](float v) { return up([](float x) { return row_warp_sum(x); }, [](float x, float y) { return x + y; }, v); };
+  auto max_up = [&](float v) {                          // of magnitudes and NaN
+    return up([](float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); },
+              [](float x, float y) { return row_max3(x, y, y); }, v);
+  };
+  // eight elements from k0 on; their type is decided once, so that the loads overlap
+  auto load8 = [&](const void* src, int dtype, int64_t at, int k0, float (&f)[8]) {
+    uint32_t u[8];
+    const int64_t i0 = at + t + static_cast<int64_t>(k0) * kThreads;
+    if (dtype == 2) {
+      const uint32_t* s = static_cast<const uint32_t*>(src) + i0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = t + (k0 + k) * kThreads < p.channels ? s[k * kThreads] : 0u;
     } else {
-      load(p.weight, p.mod_dtype, 0, w);
+      const uint16_t* s = static_cast<const uint16_t*>(src) + i0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = t + (k0 + k) * kThreads < p.channels ? s[k * kThreads] : 0u;
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      f[k] = dtype == 0 ? __uint_as_float(u[k] << 16) : (dtype == 1 ? __half2float(__ushort_as_half(static_cast<unsigned short>(u[k]))) : __uint_as_float(u[k]));
+  };
+  float z[NE];
+  const int64_t x0 = b * p.x_sb + l * p.x_sl, add0 = b * p.add_sb + l * p.add_sl, sum0 = b * p.sum_sb + l * p.sum_sl;
+#pragma unroll
+  for (int k0 = 0; k0 < NE; k0 += 8) {
+    float x[8], v[8], g[8];
+    load8(p.x, p.x_dtype, x0, k0, x);
+    if (kIsNorm<kOp> && p.add != nullptr) {
+      load8(p.add, p.add_dtype, add0, k0, v);
+      if constexpr (kOp == kRowLn) load8(p.gate, p.mod_dtype, b * p.gate_sb, k0, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = kOp == kRowLn ? fmaf(g[k], v[k], x[k]) : v[k] + x[k];
+        if (t + (k0 + k) * kThreads < p.channels) row_store(p.sum, p.sum_dtype, sum0 + t + (k0 + k) * kThreads, x[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k0 + k] = row_act<kActOf<kOp>>(x[k]);     // 0 beyond the row
+  }
+  if constexpr (kIsNorm<kOp>) {
     const float inv_c = 1.f / static_cast<float>(p.channels);
     if constexpr (kOp == kRowLn) {
       float s = 0.f;
-      each([&](int k, int) { s += z[k]; });
-      const float mean = row_block_sum(s, red, turn) * inv_c;
-      each([&](int k, int) { z[k] -= mean; });
+#pragma unroll
+      for (int k = 0; k < NE; ++k) s += z[k];
+      const float mean = sum_up(s) * inv_c;
+#pragma unroll
+      for (int k = 0; k < NE; ++k)
+        if (t + k * kThreads < p.channels) z[k] -= mean;
     }
     float s = 0.f;
-    each([&](int k, int) { s = fmaf(z[k], z[k], s); });
-    const float r = rsqrtf(row_block_sum(s, red, turn) * inv_c + p.eps);
-    each([&](int k, int) { z[k] = kOp == kRowLn ? fmaf(z[k] * r, 1.f + w[k], v[k]) : z[k] * r * w[k]; });
-  } else {
-    each([&](int k, int) { z[k] = row_act<kActOf<kOp>>(z[k]); });
+#pragma unroll
+    for (int k = 0; k < NE; ++k) s = fmaf(z[k], z[k], s);
+    const float r = rsqrtf(sum_up(s) * inv_c + p.eps);
+#pragma unroll
+    for (int k0 = 0; k0 < NE; k0 += 8) {
+      float w[8], v[8];
+      load8(kOp == kRowRms ? p.weight : p.scale, p.mod_dtype, kOp == kRowRms ? 0 : b * p.scale_sb, k0, w);
+      if constexpr (kOp == kRowLn) load8(p.shift, p.mod_dtype, b * p.shift_sb, k0, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k0 + k] = kOp == kRowLn ? fmaf(z[k0 + k] * r, 1.f + w[k], v[k]) : z[k0 + k] * r * w[k];   // 0 beyond
+    }
   }
   float top = 0.f;
-  each([&](int k, int) { top = row_max3(top, z[k], z[k]); });
-  const RowScale rs = row_scale_of(row_block_max(__float_as_uint(top), red, turn));
-  const bool zeros = rs.inverse == 0.f;
-  int8_t* q = p.q + row * p.q_stride;
-  each([&](int k, int c) { q[c] = static_cast<int8_t>(zeros ? 0u : row_quantize(z[k], rs.inverse) & 0xffu); });
+#pragma unroll
+  for (int k = 0; k < NE; k += 2) top = row_max3(top, z[k], z[k + 1]);
+  const RowScale rs = row_scale_of(__float_as_uint(max_up(top)));
+  int8_t* q = p.q + row * p.q_stride + t;
+  if (rs.inverse == 0.f) {
+#pragma unroll
+    for (int k = 0; k < NE; ++k)
+      if (t + k * kThreads < p.channels) q[k * kThreads] = 0;
+  } else {
+#pragma unroll
+    for (int k = 0; k < NE; ++k)
+      if (t + k * kThreads < p.channels) q[k * kThreads] = static_cast<int8_t>(row_quantize(z[k], rs.inverse));
+  }
   if (t == 0) p.row_scale[row] = rs.scale;
 }
 
@@ -475,7 +522,7 @@ __global__ void __launch_bounds__(kRowThreads) int8_row_any_kernel(const Int8Row
   grid_launch_dependents();
   int turn = 0;
   const int64_t row = blockIdx.x;
-  const int64_t b = row / p.seqlen, l = row % p.seqlen;
+  const int64_t b = blockIdx.x / static_cast<unsigned>(p.seqlen), l = blockIdx.x % static_cast<unsigned>(p.seqlen);
   const int64_t x0 = b * p.x_sb + l * p.x_sl, add0 = b * p.add_sb + l * p.add_sl, sum0 = b * p.sum_sb + l * p.sum_sl;
   const float inv_c = 1.f / static_cast<float>(p.channels);
   auto z_at = [&](int c) -> float {
@@ -547,14 +594,25 @@ int8_dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, vo
   }
 }
 
+// The same for rows that start anywhere, eight single elements per lane.
+constexpr int kDequantizeSingles = 8 * 32;
 __global__ void __launch_bounds__(kRowThreads)
-int8_dequantize_any_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int dtype, int channels) {
+int8_dequantize_any_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t out_stride, int dtype, int64_t rows, int channels,
+                           int pieces) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t row = blockIdx.x;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = unit / pieces;
+  if (row >= rows) return;
+  const int c0 = static_cast<int>(unit - row * pieces) * kDequantizeSingles + (threadIdx.x & 31);
   const float s = scale[row];
-  for (int c = threadIdx.x; c < channels; c += kRowThreads)
-    row_store(out, dtype, row * out_stride + c, static_cast<float>(q[row * q_stride + c]) * s);
+  const int8_t* src = q + row * q_stride;
+  int v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c0 + 32 * j < channels ? src[c0 + 32 * j] : 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c0 + 32 * j < channels) row_store(out, dtype, row * out_stride + c0 + 32 * j, static_cast<float>(v[j]) * s);
 }
 
 }  // namespace dmf

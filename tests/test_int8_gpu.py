@@ -85,6 +85,24 @@ def test_ln_modulate(C, stream, dtype, mod):
         assert z.dtype == stream and bool(((z.double() - z_ref).abs() <= near).all())
 
 
+@pytest.mark.parametrize("C", [511, 513, 777, 1023, 1153, 1535, 1919, 2047, 4001, 4095, 8191, 8193])
+def test_odd_widths(C):
+    """rows an element at a time: one, two, four and eight warps on a row, and what is wider; 21 rows fill no block"""
+    x, h, res = _randn(21, C, dtype=BF16) + 0.25, _randn(21, C, dtype=BF16, seed=1), _randn(21, C, seed=2)
+    for act in (None, "gelu", "silu"):
+        _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U if act else 0.0)
+    w = 1 + _randn(C, std=0.2, seed=3)
+    rows, z = rms_norm_int8(h, w.half(), residual=res)
+    _check_rows(rows, orc.rms_norm(h, w.half(), 1e-6, res)[0], _norm_error(C))
+    assert torch.equal(z, res + h.float())
+    mods = _randn(3, 1, 6 * C, dtype=BF16, seed=4, std=0.4)
+    gate, shift, scale = mods.chunk(6, dim=-1)[2:5]
+    x3, h3 = x.view(3, 7, C), h.view(3, 7, C)
+    rows, z = ln_modulate_int8(x3, shift, scale, gate=gate, h=h3)
+    _check_rows(rows, orc.ln_modulate(x3, shift, scale, 1e-6, gate, h3)[0], _norm_error(C))
+    assert torch.equal(rows.dequantize(F32), rows.values.float() * rows.scale[..., None])
+
+
 def test_rows_of_zeros_tiny_values_and_large_ones():
     x = _randn(7, 96, std=1.0)
     x[0] = 0.0
@@ -188,7 +206,7 @@ def _check_linear(x, w, bias, out_dtype):
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 16, 1), (1, 1152, 6912), (2, 48, 130), (5, 33, 7), (16, 1152, 384), (17, 100, 129), (64, 384, 300),
                  (128, 128, 128), (130, 1001, 258), (256, 4608, 1152), (257, 640, 513), (300, 31, 1000), (1000, 1152, 200),
-                 (2049, 144, 776), (4000, 1152, 1152)]
+                 (2049, 144, 776), (4000, 1152, 1152), (8200, 256, 1152), (5000, 128, 3456), (20000, 130, 1100), (19000, 64, 257)]
 
 
 @pytest.mark.parametrize("shape", LINEAR_SHAPES)
