@@ -19,6 +19,7 @@ namespace {
 using namespace dmf;
 
 constexpr int kMaxK = 131071;  // 128 * 128 * K stays below 2^31
+constexpr int kMaxN = 1 << 30;  // the columns of a last tile stay in int
 
 // ---- the product on the tensor cores ----
 
@@ -194,7 +195,7 @@ int run_linear_any(const dmf_int8_linear_args* a) {
 int run_linear(const dmf_int8_linear_args* a) {
   if (a == nullptr) return DMF_ATTN_ERR_NULL;
   if (!known_dtype(a->out_dtype) || (a->bias != nullptr && !known_dtype(a->bias_dtype))) return DMF_ATTN_ERR_DTYPE;
-  if (a->m < 0 || a->n < 1 || a->k < 1 || a->k > kMaxK) return DMF_ATTN_ERR_SHAPE;
+  if (a->m < 0 || a->n < 1 || a->n > kMaxN || a->k < 1 || a->k > kMaxK) return DMF_ATTN_ERR_SHAPE;
   int sms = 0, st = DMF_ATTN_OK;
   if (a->m > 0) {
     if ((st = check_matrix(a->x, a->k, false)) != DMF_ATTN_OK) return st;

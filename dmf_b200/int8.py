@@ -29,6 +29,7 @@ from . import ops as _ops
 
 _DTYPES = {torch.bfloat16: _lib.INT8_BF16, torch.float16: _lib.INT8_FP16, torch.float32: _lib.INT8_F32}
 MAX_ROWS, MAX_WIDTH = 2 ** 31 - 1, 2 ** 20
+MAX_N = 2 ** 30     # rows of a weight
 MAX_K = 131071      # of a product: beyond it a sum of 8-bit products could leave int32
 
 
@@ -390,6 +391,8 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
         raise ValueError(f"x (..., K) and weight (N, K) do not fit: {tuple(x.values.shape)} and {tuple(weight.values.shape)}")
     if x.values.shape[-1] > MAX_K:
         raise ValueError(f"rows of at most {MAX_K} elements: longer sums could leave int32")
+    if weight.values.shape[0] > MAX_N:
+        raise ValueError(f"a weight of at most {MAX_N} rows")
     if out_dtype not in _DTYPES:
         raise TypeError(f"out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
     if weight.values.device != x.values.device:

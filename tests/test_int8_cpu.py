@@ -63,6 +63,9 @@ def test_refusals(cuda_shapes):
         (ValueError, lambda: int8_linear(r8(3, 64), r8(0, 64))),
         (ValueError, lambda: int8_linear(r8(3, 64), r8(5, 64), t(4))),
         (ValueError, lambda: int8_linear(r8(3, MAX_K + 1), r8(5, MAX_K + 1))),
+        (ValueError, lambda: int8_linear(r8(3, 1), r8(2 ** 30 + 1, 1))),
+        (ValueError, lambda: quantize_int8(t(2, 2 ** 20 + 1))),
+        (ValueError, lambda: quantize_int8(t(2 ** 31, 1))),
         (TypeError, lambda: int8_linear(r8(3, 64), r8(5, 64), out_dtype=torch.int32)),
         (TypeError, lambda: int8_linear(r8(3, 64), r8(5, 64), t(5, dtype=torch.int32))),
         (TypeError, lambda: int8_linear(Int8Rows(t(3, 64), t(3, dtype=torch.float32)), r8(5, 64))),
@@ -119,7 +122,7 @@ def test_linear_rejects_bad_arguments():
         a.x, a.w = _lib.Int8Matrix(FAKE, 64, FAKE), _lib.Int8Matrix(FAKE, 64, FAKE)
         a.out, a.out_stride = FAKE, 5
         return a
-    for change, status in [(dict(m=-1), 5), (dict(n=0), 5), (dict(k=0), 5), (dict(k=131072), 5), (dict(out_dtype=3), 2),
+    for change, status in [(dict(m=-1), 5), (dict(n=0), 5), (dict(k=0), 5), (dict(k=131072), 5), (dict(n=(1 << 30) + 1, out_stride=1 << 31), 5), (dict(out_dtype=3), 2),
                            (dict(bias=FAKE, bias_dtype=7), 2), (dict(bias=FAKE + 1), 7), (dict(out=None), 1), (dict(out=FAKE + 1), 7),
                            (dict(out_stride=4), 6), (dict(x=_lib.Int8Matrix(None, 64, FAKE)), 1), (dict(x=_lib.Int8Matrix(FAKE, -1, FAKE)), 6),
                            (dict(w=_lib.Int8Matrix(FAKE, 64, None)), 1)]:
