@@ -87,15 +87,16 @@ struct GemmPlan {
   int splits;
 };
 
-// The cut with the shortest time by a model of it in microseconds, fitted to measurements of all of them at 43 shapes of 1 to
-// 16384 rows (K 128 to 8192, N 100 to 8192), where its choice is 3 % above the best on average and 24 % at most.  A step of k costs
-// what its loads take at the 102 GB/s per SM that the L2 feeds all SMs with; the rest is start and end of a tile, and the exchange
-// of the sums of a split k.  Measured at the turning points: 512 x 1152 x 3456 pairs of 128 6.6 us, of 256 7.7, few rows of 64
-// 9.7; 16384 x 1152 x 3456 pairs of 256 51, of 192 56, of 128 66; 16 x 4608 x 1152 few rows of 16 in one piece 10.4, in eight 4.4.
+// The cut with the shortest time by a model of it in microseconds, fitted to measurements of all of them at 38 shapes of 1 to
+// 16384 rows (K 128 to 8192, N 100 to 8192), where its choice is 1 % above the best on average and 11 % at most.  A step of k costs
+// what its loads take: their latency over the stages in flight for a CTA alone, the 100 to 115 GB/s that the L2 gives an SM for
+// several; the rest is start and end of a tile, and the exchange of the sums of a split k.  Measured at the turning points:
+// 512 x 1152 x 3456 pairs of 128 6.6 us, of 256 7.7, few rows of 64 9.7; 16384 x 1152 x 3456 pairs of 256 51, of 192 56, of 128 66;
+// 1024 x 1152 x 1152 few rows of 64 5.7, pairs of 128 6.1; 16 x 4608 x 1152 few rows of 16 in one piece 10.0, in eight 4.6.
 //   pair: rounds of tiles over the SM pairs, each c(bn) + steps * t(bn); a last round that is partly empty runs faster, so the
 //         rounds are halfway between the whole and the fractional number
-//   few:  tiles per SM, each e(tb) + steps / splits * (128 + tb) * 128 bytes; splits only where every CTA has an SM of its own,
-//         for 0.4 + 0.0007 per CTA and column sent
+//   few:  n tiles per SM, two at a time, each e(tb) and its steps; splits only where every CTA has an SM of its own, for 1.1 + 0.0007
+//         per CTA and column sent
 GemmPlan plan_gemm(int m, int n, int k, int sms) {
   const double steps = (k + 127) / 128;
   auto tiles = [&](int tm, int tn) { return static_cast<double>((static_cast<int64_t>(m) + tm - 1) / tm) * static_cast<double>((static_cast<int64_t>(n) + tn - 1) / tn); };
@@ -112,13 +113,13 @@ GemmPlan plan_gemm(int m, int n, int k, int sms) {
     const double rounds = (tiles(256, g.bn) - (narrow_end(n, g.bn) ? 0.4 * tiles(256, n) : 0.0)) / (sms / 2);
     consider(false, g.bn, 1, 3.4 + (std::fmax(rounds, 1.0) + std::ceil(rounds)) / 2 * (g.c + steps * g.t));
   }
-  struct { int tb; double e; } fews[] = {{16, 0.55}, {32, 1.4}, {64, 3.2}};
+  struct { int tb; double e; } fews[] = {{16, 0.1}, {32, 0.25}, {64, 0.9}};
   for (const auto& g : fews)
     for (int s = 1; s <= 8 && s <= steps; s *= 2) {
-      const double count = tiles(g.tb, 128) * s;
+      const double count = tiles(g.tb, 128) * s, n = std::ceil(count / sms), waves = std::ceil(n / 2), own = std::ceil(steps / s);
       if (s > 1 && count > sms) break;
-      consider(true, g.tb, s, 2.7 + std::ceil(count / sms) * (g.e + std::ceil(steps / s) * (128 + g.tb) * 128 / 102e3) +
-                                  (s > 1 ? 0.4 + 0.0007 * count * g.tb * (s - 1) / s : 0.0));
+      consider(true, g.tb, s, 2.3 + n * g.e + std::fmax(waves * own * 0.213, n * own * (128 + g.tb) * 128 / 115e3) + 2.0 * (waves - 1) +
+                                  (s > 1 ? 1.1 + 0.0007 * count * g.tb * (s - 1) / s : 0.0));
     }
   return best;
 }

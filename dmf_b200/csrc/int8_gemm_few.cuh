@@ -6,9 +6,10 @@
 // shared memory; after one cluster barrier CTA r adds up columns [r TB / S, (r + 1) TB / S), scales them and writes them, 32
 // consecutive channels of a token per warp instruction.
 //
-// What bounds it: latency.  Of the 4.8 us that 1 x 1152 x 6912 takes, 1.2 are the weight's 8 MB at the HBM's rate; 3.2 us is what 3
-// steps of k take in one tile, and every further step 0.2.  A cluster costs 0.4 to 3 us, so only long sums are split: 16 x 4608 x
-// 1152 takes 10.4 us in one piece and 4.4 in eight.  (Bulk copies between the CTAs instead of stores: 2 us more.)
+// What bounds it: latency.  Of the 4.5 us that 1 x 1152 x 6912 takes, 1.2 are the weight's 8 MB at the HBM's rate; 2.9 us is what 3
+// steps of k take in one tile, and every further step 0.21 (three to five stages in flight).  A split k costs 1 to 4 us, so only long
+// sums are split: 16 x 4608 x 1152 takes 10.0 us in one piece and 4.6 in eight.  (Bulk copies between the CTAs instead of stores: 2
+// us more; CTAs of a cluster on SMs of their own: clusters of four do not fill the GPU, 6.3 -> 11.3 us at 64 x 4608 x 1152.)
 #pragma once
 
 #include <type_traits>
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t s_ring = smem_u32(smem);
   int* sums = reinterpret_cast<int*>(smem + TR::kRingBytes);     // [source CTA][channel][column of mine]
-  float* s_x = reinterpret_cast<float*>(smem + TR::kRingBytes + TR::kSumBytes);   // the tokens' scales
+  float* s_x = reinterpret_cast<float*>(smem + TR::kRingBytes + TR::kSumBytes);   // the tokens' scales (16-byte aligned)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TR::kRingBytes + TR::kSumBytes + TB * 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + TR::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -120,13 +121,10 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
     ok = __all_sync(0xffffffffu, mbar_wait(bar(TR::kBarAcc), 0, abort_flag, p.status_word, kRoleInt8Epilogue + TR::kBarAcc));
     tc_fence_after_sync();
   }
-  auto put = [&](int col, int sum) {
-    const float y = fmaf(static_cast<float>(sum) * s_x[col], ws, b);
-    if (mine && m0 + col < p.m) {
-      T* dst = out + static_cast<int64_t>(m0 + col) * p.out_stride;
-      if constexpr (std::is_same<T, float>::value) *dst = y;
-      else *dst = T(y);
-    }
+  auto scaled = [&](int sum, float x_scale) { return fmaf(static_cast<float>(sum) * x_scale, ws, b); };
+  auto store = [&](T* dst, float y) {
+    if constexpr (std::is_same<T, float>::value) *dst = y;
+    else *dst = T(y);
   };
   constexpr int kChunk = TB < 32 ? TB : 32;
   const int cols = TB / splits, shift = __ffs(cols) - 1;   // columns of a CTA: a power of two, 2 at least
@@ -140,8 +138,23 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
       else tmem_ld_x32(lane_base + c0, v);
       tmem_wait_ld();
       if (splits == 1) {
+        // all scales before the first store, which they would otherwise wait for (64 tokens: 3.2 us of epilogue)
+        float y[kChunk];
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) put(c0 + j, static_cast<int>(v[j]));
+        for (int j = 0; j < kChunk; j += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(s_x + c0 + j);
+          y[j] = scaled(static_cast<int>(v[j]), x.x);
+          y[j + 1] = scaled(static_cast<int>(v[j + 1]), x.y);
+          y[j + 2] = scaled(static_cast<int>(v[j + 2]), x.z);
+          y[j + 3] = scaled(static_cast<int>(v[j + 3]), x.w);
+        }
+        if (mine) {
+          T* dst = out + static_cast<int64_t>(m0 + c0) * p.out_stride;
+          const int count = min(kChunk, p.m - m0 - c0);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j, dst += p.out_stride)
+            if (j < count) store(dst, y[j]);
+        }
       } else {
         // to the column's owner, columns of one channel side by side; tokens that are none travel too, nobody reads them
         auto at = [&](int c) -> uint32_t {
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(kInt8FewThreads) int8_gemm_few_kernel(const __
       for (int c = 0; c < cols && m0 + rank * cols + c < p.m; ++c) {
         int s = 0;
         for (int r = 0; r < splits; ++r) s += sums[(r * 128 + channel) * cols + c];
-        put(rank * cols + c, s);
+        if (mine) store(out + static_cast<int64_t>(m0 + rank * cols + c) * p.out_stride, scaled(s, s_x[rank * cols + c]));
       }
   }
   __syncwarp();
