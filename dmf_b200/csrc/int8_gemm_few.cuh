@@ -7,7 +7,7 @@
 // consecutive channels of a token per warp instruction.
 //
 // What bounds it: latency.  Of the 4.5 us that 1 x 1152 x 6912 takes, 1.2 are the weight's 8 MB at the HBM's rate; 2.9 us is what 3
-// steps of k take in one tile, and every further step 0.21 (three to five stages in flight).  A split k costs 1 to 4 us, so only long
+// steps of k take in one tile, and every further step 0.21 (18 to 24 KB at the 90 to 115 GB/s that an SM takes in from the L2).  A split k costs 1 to 4 us, so only long
 // sums are split: 16 x 4608 x 1152 takes 10.0 us in one piece and 4.6 in eight.  (Bulk copies between the CTAs instead of stores: 2
 // us more; CTAs of a cluster on SMs of their own: clusters of four do not fill the GPU, 6.3 -> 11.3 us at 64 x 4608 x 1152.)
 #pragma once

@@ -4,7 +4,7 @@
 //
 // A block owns 64 x 64 outputs, a thread 4 x 4 of them; 64 bytes of k at a time lie in shared memory as words of four, which
 // dp4a multiplies and adds to int32.  Bytes are read one by one.  16384 x 1152 x 3456 takes 1.7 ms here, against 51 us on the tensor
-// cores: rows that this package makes start at multiples of 16 bytes.
+// cores: rows that this package makes start at multiples of 16 bytes, and the callers above the C entry copy others for large products.
 #pragma once
 
 #include <stdint.h>

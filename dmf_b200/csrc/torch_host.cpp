@@ -1200,6 +1200,20 @@ MatrixView matrix_view(const Tensor& values, const Tensor& scale) {
   return v;
 }
 
+// int8.COPY_FROM: from here on a product is worth a copy of rows that the tensor cores cannot read
+constexpr double kInt8CopyFrom = 268435456.0;
+
+// rows that start at multiples of 16 bytes
+void pitch_rows(MatrixView* v) {
+  if (reinterpret_cast<uintptr_t>(v->m.values) % 16 == 0 && (v->rows == 1 || v->m.stride % 16 == 0)) return;
+  const int64_t pitch = int8_pitch(v->k);
+  const Tensor out(at::detail::empty_strided_cuda({v->rows, v->k}, {pitch, 1}, at::kChar, v->values.device()));
+  out.copy_(v->values.as_strided({v->rows, v->k}, {v->m.stride, 1}));
+  v->values = out;
+  v->m.values = static_cast<int8_t*>(out.data_ptr());
+  v->m.stride = pitch;
+}
+
 std::optional<Tensor> int8_linear(const Tensor& xq, const Tensor& x_scale, const Tensor& wq, const Tensor& w_scale,
                                   const std::optional<Tensor>& bias_, at::ScalarType out_dtype) {
   if (!int8_route() || !is_rows8(xq, x_scale) || !is_rows8(wq, w_scale) || !int8_takes(bias_, xq) || int8_dtype(out_dtype) < 0 ||
@@ -1211,7 +1225,11 @@ std::optional<Tensor> int8_linear(const Tensor& xq, const Tensor& x_scale, const
   if (status_word == nullptr) return std::nullopt;
   at::AutoDispatchBelowADInplaceOrView below_autograd;
   const c10::cuda::CUDAGuard device_guard(xq.device());
-  const MatrixView x = matrix_view(xq, x_scale), w = matrix_view(wq, w_scale);
+  MatrixView x = matrix_view(xq, x_scale), w = matrix_view(wq, w_scale);
+  if (static_cast<double>(x.rows) * w.rows * x.k >= kInt8CopyFrom) {
+    pitch_rows(&x);
+    pitch_rows(&w);
+  }
   Tensor bias;
   c10::SmallVector<int64_t, 8> shape(xq.sizes().begin(), xq.sizes().end());
   shape.back() = w.rows;

@@ -2,7 +2,7 @@
 channel, and the norms in front of them with their result in that form.
 
     rows = ln_modulate_int8(x, shift, scale)          # or rms_norm_int8, quantize_int8
-    y = int8_linear(rows, weight, bias)               # weight = quantize_int8(linear.weight), once
+    y = int8_linear(rows, weight, bias)               # weight = quantize_int8(linear.weight.detach()), once
 
 The reference samples with 16-bit linear layers (models/layers.py:119-201); on a B200 their products are most of a sampling
 step, and the tensor cores multiply 8-bit integers at twice the 16-bit rate.  ``harness.int8_model`` puts the layers of a DMFT
@@ -35,7 +35,8 @@ MAX_K = 131071      # of a product: beyond it a sum of 8-bit products could leav
 
 class Int8Rows(NamedTuple):
     """Rows in 8 bits: ``values`` (..., C) int8 and ``scale`` (...) fp32; an element stands for value * scale of its row.
-    The ops return values whose rows start at multiples of 16 bytes, which the tensor-core product reads directly."""
+    The ops return values whose rows start at multiples of 16 bytes, which the tensor-core product reads directly; a large
+    product of other rows copies them first."""
 
     values: torch.Tensor
     scale: torch.Tensor
@@ -202,10 +203,25 @@ def _matrix8(values: torch.Tensor) -> torch.Tensor:
     return v if v.stride(1) == 1 or v.shape[1] == 1 else v.contiguous()
 
 
+# Products of this many terms and more are worth a copy of rows that the tensor cores cannot read: the integer pipe, which reads any
+# row, adds up 4e13 terms a second, and a copy takes a few microseconds.
+COPY_FROM = 2 ** 28
+
+
+def _pitched(v: torch.Tensor) -> torch.Tensor:
+    """(M, K) int8 with rows that start at multiples of 16 bytes."""
+    if v.data_ptr() % 16 == 0 and (v.shape[0] == 1 or v.stride(0) % 16 == 0):
+        return v
+    out = torch.empty_strided(v.shape, (_pitch(v.shape[1]), 1), dtype=torch.int8, device=v.device)
+    return out.copy_(v)
+
+
 def int8_linear_raw(xq, x_scale, wq, w_scale, bias, out_dtype: torch.dtype):
     N, K = wq.shape
     with torch.cuda.device(xq.device):
         x2, w2 = _matrix8(xq), _matrix8(wq)
+        if x2.shape[0] * N * K >= COPY_FROM:
+            x2, w2 = _pitched(x2), _pitched(w2)
         x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
         bias = None if bias is None else bias.contiguous()
         out = torch.empty((*xq.shape[:-1], N), dtype=out_dtype, device=xq.device)

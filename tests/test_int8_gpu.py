@@ -206,7 +206,7 @@ def _check_linear(x, w, bias, out_dtype):
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 16, 1), (1, 1152, 6912), (2, 48, 130), (5, 33, 7), (16, 1152, 384), (17, 100, 129), (64, 384, 300),
                  (128, 128, 128), (130, 1001, 258), (256, 4608, 1152), (257, 640, 513), (300, 31, 1000), (1000, 1152, 200),
-                 (2049, 144, 776), (4000, 1152, 1152), (8200, 256, 1152), (5000, 128, 3456), (20000, 130, 1100), (19000, 64, 257)]
+                 (2049, 144, 776), (4000, 1152, 1152), (8200, 256, 1152), (5000, 128, 3456), (20000, 130, 1100), (19000, 64, 257), (2000, 1001, 300), (1, 100003, 2700)]
 
 
 @pytest.mark.parametrize("shape", LINEAR_SHAPES)
@@ -262,6 +262,22 @@ def test_dequantize(C, dtype):
     for r in (_random8(33, C), _pitched(_random8(33, C)), _random8(2, 3, C), quantize_int8(_randn(3, 5, C))):
         out = r.dequantize(dtype)
         assert out.is_contiguous() and torch.equal(out, (r.values.float() * r.scale[..., None]).to(dtype))
+
+
+def test_large_products_of_rows_the_tensor_cores_cannot_read():
+    """sliced columns, an odd base, expanded rows and leading dimensions that do not collapse: the result of rows side by side"""
+    K, N = 600, 500
+    big, w = _random8(1200, K + 40), _random8(N, K, seed=1)
+    ref_w = _pitched(w)
+    base = torch.empty(N * K + 5, dtype=torch.int8, device=DEV)[5:].view(N, K).copy_(w.values)
+    for x in (Int8Rows(big.values[:, 3:K + 3], big.scale), Int8Rows(big.values[:, :K], big.scale),
+              Int8Rows(big.values[:1, :K].expand(1200, K), big.scale),
+              Int8Rows(big.values.view(4, 300, -1).transpose(0, 1)[..., 1:K + 1], big.scale.view(4, 300).t())):
+        ref = int8_linear(_pitched(Int8Rows(x.values.contiguous(), x.scale.contiguous())), ref_w)
+        for weight in (w, ref_w, Int8Rows(base, w.scale)):
+            assert torch.equal(int8_linear(x, weight), ref)
+            flat = Int8Rows(x.values.reshape(-1, K), x.scale.reshape(-1))
+            assert torch.equal(torch.ops.dmf_b200.int8_linear(*flat, *weight, None, BF16).view(ref.shape), ref)
 
 
 def test_rows_behind_the_last_one_stay_as_they_were():
