@@ -416,6 +416,50 @@ def test_another_stream_and_a_graph():
     assert all(torch.equal(o, want) for _, o in graphs)
 
 
+def test_a_graph_that_forks_and_joins():
+    """operands made on two streams, one behind the package's own kernels and one behind torch's, and used behind the join"""
+    x, w = _randn(3000, 1152, dtype=BF16), _randn(640, 1152, dtype=BF16, seed=1)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def both(x, w, side):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            rows = quantize_int8(quantize_int8(x, "gelu").dequantize() * 2, "silu")
+        weight = quantize_int8(rms_norm_int8(w, torch.ones(1152, device=DEV)).dequantize())
+        main.wait_stream(side)
+        return int8_linear(rows, weight), int8_linear(rows, weight, out_dtype=F32)
+    with torch.cuda.graph(graph):
+        out = both(x, w, side)
+    for i in range(10):
+        x.copy_(_randn(3000, 1152, dtype=BF16, seed=10 + i))
+        w.copy_(_randn(640, 1152, dtype=BF16, seed=50 + i))
+        graph.replay()
+        got = [o.clone() for o in out]
+        rows = quantize_int8(quantize_int8(x, "gelu").dequantize() * 2, "silu")
+        torch.cuda.synchronize()
+        weight = quantize_int8(rms_norm_int8(w, torch.ones(1152, device=DEV)).dequantize())
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], int8_linear(rows, weight)) and torch.equal(got[1], int8_linear(rows, weight, out_dtype=F32))
+
+
+def test_many_calls_in_a_row_reuse_memory():
+    """calls whose buffers the allocator hands on at once: each kernel starts while the one before it ends"""
+    x = [_randn(m, 384, dtype=BF16, seed=m) for m in (7, 300, 1500, 5000)]
+    w = quantize_int8(_randn(384, 384))
+    want = []
+    for t in x:
+        for _ in range(3):
+            t = int8_linear(quantize_int8(t, "gelu"), w)
+            torch.cuda.synchronize()
+        want.append(t)
+    for _ in range(20):
+        for t, ref in zip(x, want):
+            for _ in range(3):
+                t = int8_linear(quantize_int8(t, "gelu"), w)
+            assert torch.equal(t, ref)
+
+
 def test_two_threads_at_once():
     import threading
     w = quantize_int8(_randn(1152, 1152))
