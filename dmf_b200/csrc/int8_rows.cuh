@@ -327,7 +327,9 @@ constexpr int kRowVectors = !kIsNorm<kOp> ? 0 : (kOp == kRowRms ? 1 : (std::is_v
 
 template <int kOp, typename TX, typename TA, int NV, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_group_kernel(const Int8RowParams p, int rows_per_block) {
-  extern __shared__ __align__(16) float s_vec[];   // kRowVectors x channels: [weight or 1 + scale | shift | gate]
+  // kRowVectors x channels: [weight or 1 + scale | shift | gate], the first halves of all eights in front of the second ones, so that
+  // a warp's 16-byte reads lie side by side
+  extern __shared__ __align__(16) float s_vec[];
   __shared__ float red[2][32];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -338,9 +340,9 @@ __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_
       float f[8];
       auto stage = [&](int which, const void* src, int64_t at, float plus) {
         row_vec8(src, p.mod_dtype, at + c, f);
-        float4* d = reinterpret_cast<float4*>(s_vec + which * p.channels + c);
-        d[0] = make_float4(f[0] + plus, f[1] + plus, f[2] + plus, f[3] + plus);
-        d[1] = make_float4(f[4] + plus, f[5] + plus, f[6] + plus, f[7] + plus);
+        float* d = s_vec + which * p.channels + (c >> 1);
+        *reinterpret_cast<float4*>(d) = make_float4(f[0] + plus, f[1] + plus, f[2] + plus, f[3] + plus);
+        *reinterpret_cast<float4*>(d + (p.channels >> 1)) = make_float4(f[4] + plus, f[5] + plus, f[6] + plus, f[7] + plus);
       };
       if constexpr (kOp == kRowRms) {
         stage(0, p.weight, 0, 0.f);
@@ -353,8 +355,8 @@ __global__ void __launch_bounds__(kWarp ? kRowThreads : kGroupThreads) int8_row_
     __syncthreads();
   }
   auto vec = [&](int which, int c, float (&f)[8]) {
-    const float4* v = reinterpret_cast<const float4*>(s_vec + (which == 0 ? 2 : which - 1) * p.channels + c);
-    const float4 a = v[0], b = v[1];
+    const float* v = s_vec + (which == 0 ? 2 : which - 1) * p.channels + (c >> 1);
+    const float4 a = *reinterpret_cast<const float4*>(v), b = *reinterpret_cast<const float4*>(v + (p.channels >> 1));
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
   };
   const int64_t per_sample = kOp == kRowLn ? p.seqlen : p.rows;
