@@ -29,9 +29,10 @@ int check_row_shape(int batch, int seqlen, int channels) {
 
 // ---- which kernel ----
 
+// rows that start at multiples of eight elements' bytes, as the kernels read and write them: 16 bytes, of fp32 32
 bool whole_vectors(const void* p, int dtype, int64_t stride_b, int batch, int64_t stride_l, int seqlen) {
-  const int64_t bytes = element_bytes(dtype);
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (batch == 1 || stride_b * bytes % 16 == 0) && (seqlen == 1 || stride_l * bytes % 16 == 0);
+  const int64_t unit = 8 * element_bytes(dtype);
+  return reinterpret_cast<uintptr_t>(p) % unit == 0 && (batch == 1 || stride_b % 8 == 0) && (seqlen == 1 || stride_l % 8 == 0);
 }
 
 bool reads_vectors(const Int8RowParams& p, int op) {

@@ -6,7 +6,7 @@
 // the loads of the next one under way while it works on the present one, and the per-channel vectors in shared memory.
 // int8_row_block_kernel has a block per row: few rows, where latency counts, and wide ones without a sample's vectors, where
 // blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 45 us
-// against 51, with GELU 66 against 78; gated LayerNorm 189 against 133).  Both move 16 bytes at a time.
+// against 51, with GELU 66 against 78; gated LayerNorm 189 against 133).  Both move eight elements at a time.
 // int8_row_single_kernel takes what these do not - odd widths, strides and alignments, mixed 16-bit types - in the same way, an
 // element at a time, and int8_row_any_kernel what is then too wide for a block's registers, computing the row again from global
 // memory in every pass.  Sums and the arithmetic are fp32.
@@ -115,14 +115,15 @@ __device__ __forceinline__ uint32_t row_block_max(uint32_t v, float (*red)[32], 
   return v;
 }
 
-// Coherent, unlike ld_nc_v4: the sum may be written where its first term was read.
+// Coherent, unlike ld_nc_v4: the sum may be written where its first term was read, and what a kernel reads may still be written by
+// the grid before it when its own blocks start (a dependent launch), which rules out non-coherent loads anywhere in these kernels.
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
-// Eight consecutive elements as they lie in memory: one 16-byte load of a 16-bit type, two of fp32.
+// Eight consecutive elements as they lie in memory: one load of 16 bytes, or of 32 for fp32.
 template <typename T>
 struct Raw8 {
   uint4 a;
@@ -133,9 +134,10 @@ struct Raw8 {
 template <>
 struct Raw8<float> {
   uint4 a, b;
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    a = ld_stream_v4(static_cast<const float*>(p) + i);
-    b = ld_stream_v4(static_cast<const float*>(p) + i + 4);
+  __device__ __forceinline__ void load(const void* p, int64_t i) {   // a whole sector per lane: two halves would be fetched twice
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(static_cast<const float*>(p) + i));
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
     const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -143,9 +145,9 @@ struct Raw8<float> {
     for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
   }
   __device__ __forceinline__ static void put(void* p, int64_t i, const float (&f)[8]) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-    d[0] = make_float4(f[0], f[1], f[2], f[3]);
-    d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(static_cast<float*>(p) + i), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
   }
 };
 
@@ -154,9 +156,9 @@ __device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, fl
   if (dtype == 0) unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + i), f);
   else if (dtype == 1) unpack8<__half>(*reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + i), f);
   else {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 a = s[0], b = s[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+                 : "l"(static_cast<const float*>(p) + i));
   }
 }
 

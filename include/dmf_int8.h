@@ -20,7 +20,7 @@
  *
  * Tensors: (B, L, C) with element strides for B and L and stride 1 for C, per-sample vectors (B, C) with an element stride for
  * B, 8-bit rows with an element stride per row (row b * L + l).  Any size from 1, any stride, any alignment that the
- * element type needs; where bases and strides are multiples of 16 bytes and C of 8 the kernels read whole vectors.
+ * element type needs; where C, strides and the bases' alignment are multiples of eight elements the kernels read whole vectors.
  *
  * Return values: the DMF_ATTN_* status codes of dmf_attn.h.  No call allocates or synchronises; zero rows launch nothing.
  */

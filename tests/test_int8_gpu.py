@@ -169,6 +169,13 @@ def test_strides_and_alignments():
     assert torch.equal(quantize_int8(sliced).values, quantize_int8(sliced.contiguous()).values)
     odd = _randn(5 * (C + 3) + 1, dtype=BF16)[1:].view(5, C + 3)[:, 1:C + 1]     # odd base and pitch
     assert torch.equal(quantize_int8(odd).values, quantize_int8(odd.contiguous()).values)
+    for shift in (1, 4):                                           # fp32 rows at 4 and at 16 bytes
+        moved = _randn(9 * C + 8)[shift:shift + 9 * C].view(9, C)
+        assert torch.equal(quantize_int8(moved).values, quantize_int8(moved.clone()).values)
+        w = torch.ones(C + 8, device=DEV)[shift:shift + C]
+        rows, z = rms_norm_int8(moved, w, residual=moved)
+        assert torch.equal(z, moved + moved)
+        _check_rows(rows, orc.rms_norm(moved, w, 1e-6, moved)[0], _norm_error(C))
     t = _randn(C, 9, dtype=BF16).t()                               # no unit stride
     assert torch.equal(quantize_int8(t).values, quantize_int8(t.contiguous()).values)
     row = _randn(C, dtype=BF16).expand(7, C)                       # one row seven times
