@@ -6,7 +6,7 @@
 // the loads of the next one under way while it works on the present one, and the per-channel vectors in shared memory.
 // int8_row_block_kernel has a block per row: few rows, where latency counts, and wide ones without a sample's vectors, where
 // blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 45 us
-// against 51, with GELU 66 against 78; gated LayerNorm 189 against 133).  Both move eight elements at a time.
+// against 51, with GELU 66 against 78; gated LayerNorm 189 against 112).  Both move eight elements at a time.
 // int8_row_single_kernel takes what these do not - odd widths, strides and alignments, mixed 16-bit types - in the same way, an
 // element at a time, and int8_row_any_kernel what is then too wide for a block's registers, computing the row again from global
 // memory in every pass.  Sums and the arithmetic are fp32.
