@@ -164,9 +164,12 @@ __device__ __forceinline__ void row_vec8(const void* p, int dtype, int64_t i, fl
 
 // row_act of eight elements, two to an instruction where there is one for two and with one reciprocal for two: 1 / d0 and 1 / d1
 // are d1 r and d0 r with r = 1 / (d0 d1), which halves the reciprocals, whose unit bounds these activations (16 results a clock
-// and SM, for them and the exponentials).  v is held at 63 so that the product stays finite; where that matters the true result is
-// below |x| 2^-63, so the caller looks at the row's maximum and takes row_act for rows below kRowActExact.
+// and SM, for them and the exponentials).  v is held at 63 so that the product stays finite; below that (|x| of 43 and more for SiLU,
+// 7.6 for GELU) the result is x 2^-63 instead of next to nothing.  Two rules keep that from the row: row_far_to_zero first puts 0 for
+// every x below kRowActFar, so that it is 2^-53 at most; and the caller takes row_act for a row whose maximum is below kRowActExact =
+// 2^-40, so that it is less than 2^-13 of the maximum and rounds to 0 like the true result.
 constexpr float kRowActExact = 9.094947017729282e-13f;   // 2^-40
+constexpr float kRowActFar = -1024.f;                    // both activations of it are below 2^-1400
 template <int kAct>
 __device__ __forceinline__ void row_act8(float (&f)[8]) {
   constexpr float kLog2e = 1.4426950408889634f, c1 = -2.f * 0.7978845608028654f * kLog2e;
@@ -181,6 +184,25 @@ __device__ __forceinline__ void row_act8(float (&f)[8]) {
     unpack_f2(add2(pack_f2(1.f, 1.f), pack_f2(fast_exp2(fminf(v0, 63.f)), fast_exp2(fminf(v1, 63.f)))), d0, d1);
     const float r = row_rcp(d0 * d1);
     unpack_f2(mul2(x, mul2(pack_f2(d1, d0), pack_f2(r, r))), f[i], f[i + 1]);
+  }
+}
+
+// 0, whose activation is 0, for each x below kRowActFar; -infinity stays, its row has no scale.  One minimum for two elements and a
+// branch that ordinary rows do not take: 16384 x 4608 bf16 behind GELU 52.7 -> 54.6 us, behind SiLU 51.3 -> 52.3 (a select per element
+// would be two instructions instead of half of one).
+template <int NV>
+__device__ __forceinline__ void row_far_to_zero(float (&z)[NV][8]) {
+  float low = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) asm("min.f32 %0, %0, %1, %2;" : "+f"(low) : "f"(z[k][i]), "f"(z[k][i + 1]));
+  if (low < kRowActFar) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (z[k][i] < kRowActFar && z[k][i] >= -3.402823466e38f) z[k][i] = 0.f;
   }
 }
 
@@ -239,6 +261,7 @@ __device__ __forceinline__ void row_in_registers(const Int8RowParams& p, RowLoad
   }
   load_next();
   if constexpr (kActOf<kOp> != 0) {
+    row_far_to_zero<NV>(z);
 #pragma unroll
     for (int k = 0; k < NV; ++k) row_act8<kActOf<kOp>>(z[k]);
   }

@@ -613,3 +613,29 @@ def test_model_refusals():
         int8_model(_model().cpu())
     with pytest.raises(ValueError, match="fp32 or bf16"):
         int8_model(_model().half())
+
+
+# Results far below their row's maximum, of large negative values: real numbers of magnitude x e^-|x|, which round to 0.  The rows: one
+# such value among ordinary ones; beside a row maximum near 2^-40 (just below, just above); nothing else (all results are below 2^-120: scale 0).
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("C", [96, 1152, 1153, 4608])
+@pytest.mark.parametrize("dtype", [BF16, F32, FP16])
+def test_activations_of_large_negative_values(act, C, dtype):
+    for M in (12, 1500):                       # a block per row; loops over rows, where there is one
+        x = _randn(M, C, std=2.0)
+        large = [-1030.0, -1e5, -1e18, -1e20, -3e38] if dtype != FP16 else [-1030.0, -6e4]
+        for r in range(M):
+            v, kind = large[r % len(large)], r % 12
+            if kind < 6:                       # one, two and half a row of them among ordinary values
+                x[r, r % C] = v
+                x[r, (5 * r + 1) % C] = v
+                if kind == 5:
+                    x[r, ::2] = v
+            elif kind < 9:                     # a row whose maximum, half of 2^-39 or 2^-40.5, is near the limit of the fast form
+                x[r] = -200.0
+                x[r, (3 * r + 2) % C] = (2.0 ** -39, 2.0 ** -38.5, 2.0 ** -40.5)[kind - 6] if dtype != FP16 else 2.0 ** -20
+                x[r, r % C] = v
+            else:
+                x[r] = v
+        x = x.to(dtype)
+        _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U)
