@@ -85,7 +85,8 @@ int launch_group(const Int8RowParams& p, int threads, int sms, cudaStream_t stre
   static bool allowed[64];
   const auto kernel = int8_row_group_kernel<kOp, TX, TA, NV, kWarp>;
   const int smem = kRowVectors<kOp, TA> * p.channels * 4;
-  if (smem > 48 * 1024 && !allow_smem(kernel, kRowVectors<kOp, TA> * kMaxEights * 32, allowed)) return DMF_ATTN_ERR_LAUNCH;
+  constexpr int kOwnWords = 2 * 32 * 4;   // the kernel's static shared memory, which counts against the 48 KB that need no leave
+  if (smem + kOwnWords > 48 * 1024 && !allow_smem(kernel, kRowVectors<kOp, TA> * kMaxEights * 32, allowed)) return DMF_ATTN_ERR_LAUNCH;
   static std::atomic<int> registers{0};
   const int st = registers_of(kernel, registers);
   if (st != DMF_ATTN_OK) return st;

@@ -639,3 +639,22 @@ def test_activations_of_large_negative_values(act, C, dtype):
                 x[r] = v
         x = x.to(dtype)
         _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U)
+
+
+@pytest.mark.parametrize("C,gated", [(4080, True), (4096, True), (6120, False), (6144, False)])
+def test_ln_modulate_as_a_programs_first_call(C, gated):
+    """vectors of just up to 48 KB in shared memory: with the block's own words more than a kernel has unless it was allowed more, which
+    an earlier and wider call of the same kernel does too; so in a program of its own"""
+    import subprocess
+    import sys
+    program = f"""
+import torch
+from dmf_b200.int8 import ln_modulate_int8
+x = torch.randn(2, 700, {C}, device="cuda").bfloat16()
+gate, shift, scale = torch.randn(2, 1, 3 * {C}, device="cuda").bfloat16().chunk(3, -1)
+rows = ln_modulate_int8(x, shift, scale, gate=gate, h=x)[0] if {gated} else ln_modulate_int8(x, shift, scale)
+few = ln_modulate_int8(x[:1, :3], shift[:1], scale[:1], gate=gate[:1], h=x[:1, :3])[0] if {gated} else ln_modulate_int8(x[:1, :3], shift[:1], scale[:1])
+assert int((rows.values[:1, :3].int() - few.values.int()).abs().max()) <= 1
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
