@@ -1203,9 +1203,9 @@ MatrixView matrix_view(const Tensor& values, const Tensor& scale) {
 // int8.COPY_FROM: from here on a product is worth a copy of rows that the tensor cores cannot read
 constexpr double kInt8CopyFrom = 268435456.0;
 
-// rows that start at multiples of 16 bytes
+// rows that start at multiples of 16 bytes and do not overlap, as the tensor-core kernels read them
 void pitch_rows(MatrixView* v) {
-  if (reinterpret_cast<uintptr_t>(v->m.values) % 16 == 0 && (v->rows == 1 || v->m.stride % 16 == 0)) return;
+  if (reinterpret_cast<uintptr_t>(v->m.values) % 16 == 0 && (v->rows == 1 || (v->m.stride % 16 == 0 && v->m.stride >= v->k))) return;
   const int64_t pitch = int8_pitch(v->k);
   const Tensor out(at::detail::empty_strided_cuda({v->rows, v->k}, {pitch, 1}, at::kChar, v->values.device()));
   out.copy_(v->values.as_strided({v->rows, v->k}, {v->m.stride, 1}));

@@ -209,8 +209,8 @@ COPY_FROM = 2 ** 28
 
 
 def _pitched(v: torch.Tensor) -> torch.Tensor:
-    """(M, K) int8 with rows that start at multiples of 16 bytes."""
-    if v.data_ptr() % 16 == 0 and (v.shape[0] == 1 or v.stride(0) % 16 == 0):
+    """(M, K) int8 with rows that start at multiples of 16 bytes and do not overlap, as the tensor-core kernels read them."""
+    if v.data_ptr() % 16 == 0 and (v.shape[0] == 1 or (v.stride(0) % 16 == 0 and v.stride(0) >= v.shape[1])):
         return v
     out = torch.empty_strided(v.shape, (_pitch(v.shape[1]), 1), dtype=torch.int8, device=v.device)
     return out.copy_(v)

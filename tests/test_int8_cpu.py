@@ -136,3 +136,13 @@ def test_linear_rejects_bad_arguments():
     d = _lib.Int8DequantizeArgs()
     d.rows, d.channels, d.x, d.out, d.out_stride = 3, 64, _lib.Int8Matrix(FAKE, 64, FAKE), FAKE, 63
     assert lib.dmf_int8_dequantize(C.byref(d)) == 6
+
+
+def test_rows_are_copied_unless_the_tensor_cores_can_read_them():
+    from dmf_b200.int8 import _pitched
+    buf = torch.arange(0, 2000, dtype=torch.int64).to(torch.int8)
+    for v in (buf[:48].expand(9, 48), buf.as_strided((9, 48), (16, 1)), buf[:9 * 50].view(9, 50), buf[1:].as_strided((9, 48), (48, 1))):
+        out = _pitched(v)
+        assert out.stride(0) == -(-v.shape[1] // 16) * 16 and out.data_ptr() % 16 == 0 and torch.equal(out, v)
+    for v in (buf[:9 * 48].view(9, 48), buf.as_strided((9, 40), (64, 1)), buf[:50].view(1, 50), buf.as_strided((1, 50), (0, 1))):
+        assert _pitched(v).data_ptr() == v.data_ptr()

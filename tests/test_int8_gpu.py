@@ -658,3 +658,18 @@ assert int((rows.values[:1, :3].int() - few.values.int()).abs().max()) <= 1
 """
     done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_large_products_of_expanded_and_overlapping_rows_copy_them():
+    """rows at a pitch of 0, or of 16 bytes and less than a row: a copy goes to the tensor cores (seen as memory that the call takes)"""
+    M, K, N = 1200, 640, 500
+    w, scale = _pitched(_random8(N, K, seed=1)), torch.rand(M, device=DEV)
+    for values in (_random8(1, K).values.expand(M, K), _random8(1, 16 * M + K).values[0].as_strided((M, K), (16, 1))):
+        ref = int8_linear(Int8Rows(values.clone(memory_format=torch.contiguous_format), scale), w)
+        for f in (lambda: int8_linear(Int8Rows(values, scale), w),
+                  lambda: torch.ops.dmf_b200.int8_linear(values, scale, *w, None, BF16)):
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            out = f()
+            assert torch.cuda.max_memory_allocated() - before >= M * N * 2 + M * K
+            assert torch.equal(out, ref)
