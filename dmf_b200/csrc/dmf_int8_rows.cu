@@ -248,7 +248,7 @@ int run_ln_modulate(const dmf_int8_ln_modulate_args* a) {
 int run_dequantize(const dmf_int8_dequantize_args* a) {
   if (a == nullptr) return DMF_ATTN_ERR_NULL;
   if (!known_dtype(a->out_dtype)) return DMF_ATTN_ERR_DTYPE;
-  if (a->rows < 0 || a->rows > 0x7fffffff || a->channels < 1) return DMF_ATTN_ERR_SHAPE;
+  if (a->rows < 0 || a->rows > 0x7fffffff || a->channels < 1 || a->channels > kMaxChannels) return DMF_ATTN_ERR_SHAPE;
   int sms = 0, st = DMF_ATTN_OK;
   if (a->rows > 0) {
     if ((st = check_matrix(a->x, a->channels, false)) != DMF_ATTN_OK) return st;

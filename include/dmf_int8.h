@@ -13,7 +13,7 @@
  *     dmf_int8_dequantize   out[m, c] = q[m, c] scale[m]
  *
  * z is used as it is summed in fp32; what is written of it (`sum`) is its rounding to the stream's type.  The sums over k are
- * exact (int32), hence K <= 131071; N <= 2^30.
+ * exact (int32), hence K <= 131071; N <= 2^30; elsewhere C <= 2^20.  At most 2^31 - 1 rows.
  *
  * These are the block's linear layers at sampling time (models/layers.py:119-154 qkv and proj, :157-167 the MLP, :187-201
  * the modulation and the adaLN forms in front of them), which the reference runs in 16 bits.

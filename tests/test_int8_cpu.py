@@ -146,3 +146,11 @@ def test_rows_are_copied_unless_the_tensor_cores_can_read_them():
         assert out.stride(0) == -(-v.shape[1] // 16) * 16 and out.data_ptr() % 16 == 0 and torch.equal(out, v)
     for v in (buf[:9 * 48].view(9, 48), buf.as_strided((9, 40), (64, 1)), buf[:50].view(1, 50), buf.as_strided((1, 50), (0, 1))):
         assert _pitched(v).data_ptr() == v.data_ptr()
+
+
+def test_dequantize_rejects_rows_that_are_too_wide():
+    lib, a = _lib.load(), _lib.Int8DequantizeArgs()
+    a.rows, a.x, a.out = 3, _lib.Int8Matrix(FAKE, 1 << 32, FAKE), FAKE
+    for channels, status in ((2 ** 20 + 1, 5), (2 ** 31 - 1, 5), (0, 5)):
+        a.channels, a.out_stride = channels, 1 << 32
+        assert lib.dmf_int8_dequantize(C.byref(a)) == status

@@ -673,3 +673,16 @@ def test_large_products_of_expanded_and_overlapping_rows_copy_them():
             out = f()
             assert torch.cuda.max_memory_allocated() - before >= M * N * 2 + M * K
             assert torch.equal(out, ref)
+
+
+def test_rows_wider_than_2_to_the_20_are_refused_on_every_route():
+    wide, ok = 2 ** 20 + 1, 2 ** 20
+    scale = torch.ones(2, device=DEV)
+    values = torch.ones(2, wide, dtype=torch.int8, device=DEV)
+    with pytest.raises(ValueError, match="at most"):
+        Int8Rows(values, scale).dequantize()
+    with pytest.raises(RuntimeError):
+        torch.ops.dmf_b200.dequantize_int8(values, scale, BF16)
+    assert bool((Int8Rows(values[:, :ok], scale).dequantize() == 1).all())
+    with pytest.raises(ValueError, match="at most"):
+        quantize_int8(torch.ones(2, wide, dtype=BF16, device=DEV))
