@@ -686,3 +686,45 @@ def test_rows_wider_than_2_to_the_20_are_refused_on_every_route():
     assert bool((Int8Rows(values[:, :ok], scale).dequantize() == 1).all())
     with pytest.raises(ValueError, match="at most"):
         quantize_int8(torch.ones(2, wide, dtype=BF16, device=DEV))
+
+
+# ---- the kernels that take many rows: from eight rows per SM on (1184 on a B200), a warp per row up to 1280 channels, a block on wider ones
+
+MANY_WIDTHS = [64, 384, 512, 520, 1152, 1280, 1288, 2040, 4608]
+
+
+@pytest.mark.parametrize("C", MANY_WIDTHS)
+@pytest.mark.parametrize("act", [None, "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, F32])
+def test_quantize_many_rows(C, act, dtype):
+    x = _randn(1511, C, dtype=dtype, std=2.0)
+    _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U if act else 0.0)
+    x = _randn(7, 3, 211, C, dtype=dtype, seed=1)[:, 1]           # samples that do not lie side by side
+    _check_rows(quantize_int8(x, act), orc.act(x, act), 16 * U if act else 0.0)
+
+
+@pytest.mark.parametrize("C", MANY_WIDTHS)
+@pytest.mark.parametrize("dtype,stream", [(BF16, BF16), (FP16, FP16), (BF16, F32), (FP16, F32), (F32, BF16), (F32, FP16), (F32, F32)])
+def test_rms_norm_many_rows(C, dtype, stream):
+    w = 1 + _randn(C, std=0.2, seed=3)
+    x, res = _randn(7, 211, C, dtype=dtype), _randn(7, 211, C, dtype=stream, seed=1)
+    _check_rows(rms_norm_int8(x, w), orc.rms_norm(x, w, 1e-6)[0], _norm_error(C))
+    rows, z = rms_norm_int8(x, w.to(dtype), 1e-3, residual=res)
+    _check_rows(rows, orc.rms_norm(x, w.to(dtype), 1e-3, res)[0], _norm_error(C))
+    assert torch.equal(z, (res.float() + x.float()).to(stream))
+
+
+@pytest.mark.parametrize("C", MANY_WIDTHS)
+@pytest.mark.parametrize("stream,dtype,mod", [(BF16, BF16, BF16), (FP16, FP16, FP16), (BF16, F32, F32), (FP16, F32, BF16), (F32, BF16, F32),
+                                              (F32, FP16, FP16), (F32, F32, BF16)])
+def test_ln_modulate_many_rows(C, stream, dtype, mod):
+    for B, L in ((5, 307), (1, 1201), (150, 8)):       # samples with vectors of their own; no block's share of rows divides 307 or 1201
+        x, h = _randn(B, L, C, dtype=stream) + 0.5, _randn(B, L, C, dtype=dtype, seed=1)
+        gate, shift, scale = _randn(B, 1, 6 * C, dtype=mod, seed=2, std=0.4).chunk(6, dim=-1)[2:5]
+        _check_rows(ln_modulate_int8(x, shift, scale), orc.ln_modulate(x, shift, scale, 1e-6)[0], _norm_error(C))
+        rows, z = ln_modulate_int8(x, shift, scale, 1e-2, gate=gate, h=h)
+        y, z_ref = orc.ln_modulate(x, shift, scale, 1e-2, gate, h)
+        _check_rows(rows, y, _norm_error(C))
+        half = torch.finfo(stream).eps / 2
+        near = half * z_ref.abs() + 2 * U * (x.double().abs() + (gate.double() * h.double()).abs()) + 2.0 ** -25
+        assert z.dtype == stream and bool(((z.double() - z_ref).abs() <= near).all())
