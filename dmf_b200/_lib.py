@@ -33,6 +33,7 @@ EXPORTS = (
     "dmf_gate_residual_fwd", "dmf_gate_residual_bwd", "dmf_gelu",
     "dmf_step_tail",
     "dmf_int8_quantize", "dmf_int8_rmsnorm", "dmf_int8_ln_modulate", "dmf_int8_linear", "dmf_int8_dequantize",
+    "dmf_int8_linear_kernel_name",
 )
 ADALN_BF16, ADALN_F32 = 0, 2
 INT8_BF16, INT8_FP16, INT8_F32 = 0, 1, 2
@@ -229,6 +230,8 @@ def load() -> C.CDLL:
         lib.dmf_attn_kernel_name_for.argtypes = [C.c_int32] * 7 + [C.c_char_p, C.c_size_t]
         lib.dmf_attn_kernel_name.restype = C.c_int
         lib.dmf_attn_kernel_name.argtypes = [C.c_int32] * 5 + [C.c_char_p, C.c_size_t]
+        lib.dmf_int8_linear_kernel_name.restype = C.c_int
+        lib.dmf_int8_linear_kernel_name.argtypes = [C.c_int32] * 3 + [C.c_char_p, C.c_size_t]
         for name in ("dmf_attn_fwd_dual", "dmf_attn_fwd", "dmf_attn_fwd_dual_f32out"):
             fn = getattr(lib, name)
             fn.restype = C.c_int
@@ -284,6 +287,13 @@ def kernel_name(op: str, seqlen_q: int, seqlen_kv: int, head_dim: int, dtype: in
         check(load().dmf_attn_kernel_name(code, *shape))
     else:
         check(load().dmf_attn_kernel_name_for(code, batch, heads, *shape))
+    return buf.value.decode()
+
+
+def int8_linear_kernel_name(m: int, n: int, k: int) -> str:
+    """The kernel template instance and the cut of k that a product of 8-bit rows, m x k x n, takes."""
+    buf = C.create_string_buffer(256)
+    check(load().dmf_int8_linear_kernel_name(m, n, k, buf, len(buf)))
     return buf.value.decode()
 
 

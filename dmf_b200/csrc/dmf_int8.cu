@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <cstdio>
 #include <cstring>
 
 #include "attn_launch.h"
@@ -210,6 +211,22 @@ int run_linear(const dmf_int8_linear_args* a) {
   return tma_can_read(a->x, a->m, a->k) && tma_can_read(a->w, a->n, a->k) ? run_gemm(a, sms) : run_linear_any(a);
 }
 
+int linear_kernel_name(int m, int n, int k, char* buf, size_t len) {
+  if (buf == nullptr || len == 0) return DMF_ATTN_ERR_NULL;
+  if (m < 1 || n < 1 || n > kMaxN || k < 1 || k > kMaxK) return DMF_ATTN_ERR_SHAPE;
+  int sms = 0;
+  if (sm_count_of_current_device(&sms) != DMF_ATTN_OK) sms = 148;
+  const GemmPlan g = plan_gemm(m, n, k, sms);
+  if (!g.few) std::snprintf(buf, len, "int8_gemm_pair_kernel<%d>%s", g.tile, narrow_end(n, g.tile) ? ", narrow end" : "");
+  else if (g.splits == 1) std::snprintf(buf, len, "int8_gemm_few_kernel<%d>", g.tile);
+  else std::snprintf(buf, len, "int8_gemm_few_kernel<%d>, k over %d CTAs", g.tile, g.splits);
+  return DMF_ATTN_OK;
+}
+
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) int dmf_int8_linear(const dmf_int8_linear_args* args) { return run_linear(args); }
+#define DMF_API extern "C" __attribute__((visibility("default")))
+DMF_API int dmf_int8_linear(const dmf_int8_linear_args* args) { return run_linear(args); }
+DMF_API int dmf_int8_linear_kernel_name(int32_t m, int32_t n, int32_t k, char* buf, size_t len) {
+  return linear_kernel_name(m, n, k, buf, len);
+}

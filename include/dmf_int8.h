@@ -123,6 +123,12 @@ int dmf_int8_ln_modulate(const dmf_int8_ln_modulate_args* args);
 int dmf_int8_linear(const dmf_int8_linear_args* args);
 int dmf_int8_dequantize(const dmf_int8_dequantize_args* args);
 
+/*
+ * Checking hook: the kernel template instance, and the cut of k, that dmf_int8_linear picks for m x k x n on the current device (on a
+ * B200 where there is none), as text, for rows that the tensor cores can read.
+ */
+int dmf_int8_linear_kernel_name(int32_t m, int32_t n, int32_t k, char* buf, size_t len);
+
 #ifdef __cplusplus
 }
 #endif
