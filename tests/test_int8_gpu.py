@@ -728,3 +728,22 @@ def test_ln_modulate_many_rows(C, stream, dtype, mod):
         half = torch.finfo(stream).eps / 2
         near = half * z_ref.abs() + 2 * U * (x.double().abs() + (gate.double() * h.double()).abs()) + 2.0 ** -25
         assert z.dtype == stream and bool(((z.double() - z_ref).abs() <= near).all())
+
+
+@pytest.mark.parametrize("step", [None, "ln_modulate", "act", "rms_norm", "linear"])
+def test_smoke_run_sees_a_wrong_result_of_every_step(step, monkeypatch):
+    """with the oracle's step off by 1 % the comparison fails"""
+    from __graft_entry__ import _smoke_int8
+    g = torch.Generator().manual_seed(1)
+    args = [torch.device(DEV)] + [torch.randn(2, n, 384, generator=g) for n in (64, 1, 1)] + [g]
+    if step is None:
+        assert _smoke_int8(*args) < 3e-3
+        return
+    true = getattr(orc, step)
+
+    def wrong(*a, **kw):
+        out = true(*a, **kw)
+        return (out[0] * 1.01, *out[1:]) if isinstance(out, tuple) else out * 1.01
+    monkeypatch.setattr(orc, step, wrong)
+    with pytest.raises(AssertionError):
+        _smoke_int8(*args)
