@@ -11,7 +11,6 @@
 #include "int8_gemm_few.cuh"
 #include "int8_gemm_pair.cuh"
 #include "int8_launch.h"
-#include "int8_launch.h"
 #include "int8_linear.cuh"
 #include "tensor_map.h"
 
@@ -91,7 +90,8 @@ struct GemmPlan {
 // The cut with the shortest time by a model of it in microseconds, fitted to measurements of all of them at 38 shapes of 1 to
 // 16384 rows (K 128 to 8192, N 100 to 8192), where its choice is 1 % above the best on average and 11 % at most.  A step of k costs
 // what its loads take: their latency over the stages in flight for a CTA alone, the 100 to 115 GB/s that the L2 gives an SM for
-// several; the rest is start and end of a tile, and the exchange of the sums of a split k.  Measured at the turning points:
+// several; the rest is start and end of a tile, and the exchange of the sums of a split k, as it is with the bank conflicts of its layout
+// (int8_gemm_few.cuh).  Measured in bursts, short of the power limit, at the turning points:
 // 512 x 1152 x 3456 pairs of 128 6.6 us, of 256 7.7, few rows of 64 9.7; 16384 x 1152 x 3456 pairs of 256 51, of 192 56, of 128 66;
 // 1024 x 1152 x 1152 few rows of 64 5.7, pairs of 128 6.1; 16 x 4608 x 1152 few rows of 16 in one piece 10.0, in eight 4.6.
 //   pair: rounds of tiles over the SM pairs, each c(bn) + steps * t(bn); a last round that is partly empty runs faster, so the

@@ -8,7 +8,10 @@
 //
 // What bounds it: latency.  Of the 4.5 us that 1 x 1152 x 6912 takes, 1.2 are the weight's 8 MB at the HBM's rate; 2.9 us is what 3
 // steps of k take in one tile, and every further step 0.21 (18 to 24 KB at the 90 to 115 GB/s that an SM takes in from the L2).  A split k costs 1 to 4 us, so only long
-// sums are split: 16 x 4608 x 1152 takes 10.0 us in one piece and 4.6 in eight.  (Bulk copies between the CTAs instead of stores: 2
+// sums are split: 16 x 4608 x 1152 takes 10.0 us in one piece and 4.6 in eight.  With wide tiles most of that is bank conflicts: `sums`
+// holds the columns of a channel side by side, so the lanes of a warp, a channel each, read and send at a stride of `cols` words - 2-way
+// conflicts at 16 tokens in eight pieces, 16-way at 32 in two, 32-way at 64 in two (shared-memory wavefronts of a CTA's reads, and those
+// that conflicts add: 157 and 64, 2133 and 1920, 8179 and 7826).  (Bulk copies between the CTAs instead of stores: 2
 // us more; CTAs of a cluster on SMs of their own: clusters of four do not fill the GPU, 6.3 -> 11.3 us at 64 x 4608 x 1152.)
 #pragma once
 

@@ -17,8 +17,8 @@
 // two columns of each eight and so reads 16 bytes of scales and bias for eight results.  (In the row layout, where every thread
 // reads those of all columns, that alone took 6 us of 59 at 16384 x 1152 x 3456.)
 //
-// 16384 x 1152 x 3456 51 us (2.5 Pop/s), x 4608 63 us (2.7), 16384 x 4608 x 1152 66 us (2.6; 5.2 or 4.3 rounds of tiles), 8192^3
-// 345 us (3.2); a larger tile would need less of the L2, but 256 x 256 twice is all the tensor memory there is.
+// In bursts: 16384 x 1152 x 3456 51 us (2.5 Pop/s; 63 call after call, at the power limit), x 4608 63 us (2.7), 16384 x 4608 x 1152 66 us
+// (2.6; 5.2 or 4.3 rounds of tiles), 8192^3 345 us (3.2); a larger tile would need less of the L2, but 256 x 256 twice is all the tensor memory there is.
 //
 // Every wait is bounded (see sm100_ptx.cuh); a role whose wait gives up leaves its loop, the others follow at their next wait,
 // all meet at the end.

@@ -5,8 +5,8 @@
 // output.  int8_row_group_kernel has a warp (rows of up to 1280 channels) or a block (wider ones, LayerNorm) take row after row,
 // the loads of the next one under way while it works on the present one, and the per-channel vectors in shared memory.
 // int8_row_block_kernel has a block per row: few rows, where latency counts, and wide ones without a sample's vectors, where
-// blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 45 us
-// against 51, with GELU 66 against 78; gated LayerNorm 189 against 112).  Both move eight elements at a time.
+// blocks that come and go keep more loads under way than the loop's 64 registers allow (16384 x 4608: quantisation 38 us
+// against 40, with GELU 55 against 68; gated LayerNorm 188 against 101).  Both move eight elements at a time.
 // int8_row_single_kernel takes what these do not - odd widths, strides and alignments, mixed 16-bit types - in the same way, an
 // element at a time, and int8_row_any_kernel what is then too wide for a block's registers, computing the row again from global
 // memory in every pass.  Sums and the arithmetic are fp32.
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : kGroupThreads) int8_row_block
 
 // Rows that cannot be read as vectors: kWarps warps on a row, NE single elements per lane, c = thread of the row + k * threads; a
 // block of eight warps has 8 / kWarps rows.  Bound by instruction issue (a load and a store for every element): quantisation of
-// 11136 x 1919 22 us, of 1920 in vectors 13, residual + RMS norm 52 and 26, gated LayerNorm 84 and 35; a block per row took 37, 70 and
+// 11136 x 1919 23 us, of 1920 in vectors 13, residual + RMS norm 52 and 25, gated LayerNorm (samples of 128 rows) 92 and 31; a block per row took 37, 70 and
 // 130, its barriers and divisions not spread over enough elements.
 template <int kOp, int NE, int kWarps>
 __global__ void __launch_bounds__(kRowThreads) int8_row_single_kernel(const Int8RowParams p) {

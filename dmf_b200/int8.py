@@ -394,7 +394,7 @@ def ln_modulate_int8(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, 
 def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = None, *,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ weight.T + bias`` of rows in 8 bits: x (..., K), weight (N, K), bias (N); the result (..., N) in ``out_dtype``.
-    The sums are exact, one rounding at the end."""
+    The sums are exact; they, their products with the two scales and the bias's addition are rounded to fp32, the result to its type."""
     (xq, x_scale), (wq, w_scale) = x, weight
     if _native.takes(xq, x_scale, wq, w_scale, bias):
         out = _native.int8_linear(xq, x_scale, wq, w_scale, bias, out_dtype)
